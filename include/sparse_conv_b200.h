@@ -277,6 +277,75 @@ SC_API sc_status sc_attention_varlen(sc_handle* h, const void* q, const void* k,
 SC_API sc_status sc_layernorm_silu(sc_handle* h, void* x, int64_t n, int32_t c, sc_dtype dtype, int32_t apply_silu,
                             float eps);
 
+/* Group norm over sparse sequences, channels last (the norm of the sparse
+ * ResBlocks and attention blocks of the TRELLIS family; no counterpart in the
+ * TS port, whose blocks use src/dense/ops/layer_norm.ts:28-60).  x is
+ * [cu_seqlens[batch], channels] with x_stride elements between rows; every
+ * (sequence, group) is normalised with the mean and the biased variance of its
+ * rows x (channels / groups) values, then times weight plus bias ([channels] in
+ * wdtype = dtype or SC_F32; either may be NULL), then SiLU if apply_silu.
+ * y [*, channels] is dense and may be x itself when x is dense.  stats, if not
+ * NULL, receives [batch][groups][2] f32 (mean, 1 / sqrt(var + eps)) for the
+ * backward call; sequences without rows leave theirs untouched.  cu_seqlens is
+ * a HOST array of batch + 1 non-decreasing offsets starting at 0.  channels <=
+ * 4096 and a multiple of groups; pointers aligned to their elements.
+ * Statistics and sums are f32, in an order fixed by the sizes alone. */
+SC_API sc_status sc_group_norm(sc_handle* h, const void* x, int64_t x_stride, const void* weight, const void* bias,
+                               void* y, float* stats, const int32_t* cu_seqlens, int32_t batch, int32_t channels,
+                               int32_t groups, float eps, int32_t apply_silu, sc_dtype dtype, sc_dtype wdtype);
+
+/* Gradients of sc_group_norm: dy [*, channels] dense; dx [*, channels] dense,
+ * dweight and dbias [channels] in wdtype, each may be NULL (not computed).  No
+ * output may overlap an input. */
+SC_API sc_status sc_group_norm_backward(sc_handle* h, const void* x, int64_t x_stride, const void* dy,
+                                        const void* weight, const void* bias, const float* stats, void* dx,
+                                        void* dweight, void* dbias, const int32_t* cu_seqlens, int32_t batch,
+                                        int32_t channels, int32_t groups, int32_t apply_silu, sc_dtype dtype,
+                                        sc_dtype wdtype);
+
+/* Arguments of the differential attention calls.  Per sequence, query row i
+ * and head h, with g = h / (heads / kv_heads):
+ *   out[i, h] = (softmax_j(scale q[i, 2h] . k[j, 2g])
+ *                - lam_h softmax_j(scale q[i, 2h+1] . k[j, 2g+1])) v[j, g]
+ * over the sequence's key rows j; with causal, query i of the sequence sees
+ * keys j <= i + len_kv - len_q.  A row that sees no key is zero (and passes no
+ * gradient).  Two maps beside the one of sc_attention_varlen; q [Nq, 2 heads,
+ * 64], k [Nkv, 2 kv_heads, 64], v [Nkv, kv_heads, 128], out [Nq, heads, 128] in
+ * dtype (bf16 or f16).  Tokens of q, k and v are q_stride, k_stride and
+ * v_stride elements apart (multiples of 8); everything else is dense; device
+ * arrays of 16-bit elements are 16-byte aligned.  lam is [lam_count] in
+ * lam_dtype (dtype or SC_F32), lam_count 1 or heads; lam NULL means lam_value
+ * for every head.  cu_seqlens_q / cu_seqlens_kv are HOST arrays of batch + 1
+ * non-decreasing offsets starting at 0. */
+typedef struct sc_diff_attention_args {
+  const void *q, *k, *v, *lam;
+  int64_t q_stride, k_stride, v_stride;
+  const int32_t *cu_seqlens_q, *cu_seqlens_kv;
+  int32_t batch, heads, kv_heads;
+  int32_t lam_count;
+  float lam_value;
+  float scale;              /* > 0, usually 1 / 8 */
+  int32_t causal;
+  sc_dtype dtype, lam_dtype;
+  /* forward: out is written; lse [2][heads][Nq] (log-sum-exp in base 2) and
+   * maps [Nq, heads, 2, 128] (each map's product), both f32, are written for
+   * the backward call, or both are NULL.  backward: lse and maps are read, out
+   * is not. */
+  void* out;
+  float* lse;
+  float* maps;
+  /* backward only: dout [Nq, heads, 128]; gradients dense in their input's
+   * type, each may be NULL (not computed); dlam [lam_count] in lam_dtype. */
+  const void* dout;
+  void *dq, *dk, *dv, *dlam;
+} sc_diff_attention_args;
+
+/* f32 accumulation and softmax statistics; weights and score gradients are
+ * rounded to dtype for the tensor cores.  Sums have a fixed order: results
+ * repeat bit for bit. */
+SC_API sc_status sc_diff_attention(sc_handle* h, const sc_diff_attention_args* args);
+SC_API sc_status sc_diff_attention_backward(sc_handle* h, const sc_diff_attention_args* args);
+
 /* ---- Halo exchange over peer memory (sharded convs on the GPUs of one node).
  * Replaces the NCCL all-to-all of the halo rows (the exchange step of a
  * Morton-sharded conv); no counterpart in the reference, whose conv runs on

@@ -59,6 +59,16 @@ class ScKmapInfo(ctypes.Structure):
                 ("halo_max", ctypes.c_int64)]
 
 
+class ScDiffAttentionArgs(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("q", "k", "v", "lam")] + \
+               [(n, ctypes.c_int64) for n in ("q_stride", "k_stride", "v_stride")] + \
+               [(n, ctypes.c_void_p) for n in ("cu_seqlens_q", "cu_seqlens_kv")] + \
+               [(n, ctypes.c_int32) for n in ("batch", "heads", "kv_heads", "lam_count")] + \
+               [("lam_value", ctypes.c_float), ("scale", ctypes.c_float), ("causal", ctypes.c_int32),
+                ("dtype", ctypes.c_int32), ("lam_dtype", ctypes.c_int32)] + \
+               [(n, ctypes.c_void_p) for n in ("out", "lse", "maps", "dout", "dq", "dk", "dv", "dlam")]
+
+
 _P = ctypes.c_void_p
 _I32 = ctypes.c_int32
 _I64 = ctypes.c_int64
@@ -96,6 +106,11 @@ _SIGNATURES = {
     "sc_conv3d_depthwise": (_I32, [_P, _P, _P, _P, _P, _P, _I32, _I32]),
     "sc_subdivide2": (_I32, [_P, _P, _I64, _P, _P, _I32, _P, _P, _P, _I64, _P]),
     "sc_attention_varlen": (_I32, [_P, _P, _P, _P, _P, _P, _P, _I32, _I32, _I32, _F, _I32]),
+    "sc_group_norm": (_I32, [_P, _P, _I64, _P, _P, _P, _P, _P, _I32, _I32, _I32, _F, _I32, _I32, _I32]),
+    "sc_group_norm_backward": (_I32, [_P, _P, _I64, _P, _P, _P, _P, _P, _P, _P, _P, _I32, _I32, _I32, _I32, _I32,
+                                      _I32]),
+    "sc_diff_attention": (_I32, [_P, ctypes.POINTER(ScDiffAttentionArgs)]),
+    "sc_diff_attention_backward": (_I32, [_P, ctypes.POINTER(ScDiffAttentionArgs)]),
     "sc_layernorm_silu": (_I32, [_P, _P, _I64, _I32, _I32, _I32, _F]),
     "sc_peer_alloc": (_I32, [_P, ctypes.c_size_t, _PP, _P]),
     "sc_peer_free": (_I32, [_P, _P]),

@@ -4,6 +4,7 @@
 // the duration of the call, enqueues on the handle's stream and returns a
 // status code; nothing throws across the boundary.
 #include "sc_common.cuh"
+#include "sc_diffattn.h"
 #include "sc_internal.h"
 
 #include <cstdio>
@@ -92,6 +93,20 @@ sc_status wrap_kmap(Handle* h, KMap* km, uint32_t flags, sc_kmap** out) {
   *out = w;
   return SC_OK;
 }
+// Runs the body of an entry point that allocates host memory.
+template <typename F>
+sc_status guarded(Handle* H, F&& body) {
+  try {
+    return body();
+  } catch (const std::bad_alloc&) {
+    H->last_error.clear();
+    return SC_ENOMEM;
+  } catch (...) {
+    H->last_error.clear();
+    return SC_ECUDA;
+  }
+}
+
 }  // namespace
 
 extern "C" {
@@ -552,6 +567,156 @@ sc_status sc_attention_varlen(sc_handle* h, const void* q, const void* k, const 
     return sc::set_error(H, SC_EINVAL, "attention: q, k, v and out must be 16-byte aligned device arrays");
   sc::DeviceGuard g(H->device);
   return sc::attention_varlen(H, q, k, v, out, cu_seqlens_q, cu_seqlens_kv, batch, num_heads, scale, dtype);
+}
+
+namespace {
+
+bool offsets_ok(const int32_t* cu, int32_t batch) {
+  if (cu[0] != 0) return false;
+  for (int32_t b = 0; b < batch; ++b)
+    if (cu[b + 1] < cu[b]) return false;
+  return true;
+}
+
+size_t dtype_bytes(sc_dtype t) { return t == SC_F32 ? 4 : 2; }
+
+sc_status gn_check(Handle* H, const void* x, int64_t x_stride, const void* weight, const void* bias,
+                   const int32_t* cu, int32_t batch, int32_t channels, int32_t groups, sc_dtype dtype,
+                   sc_dtype wdtype) {
+  if (dtype != SC_F32 && dtype != SC_BF16 && dtype != SC_F16)
+    return sc::set_error(H, SC_EINVAL, "group norm: unknown dtype");
+  if (wdtype != dtype && wdtype != SC_F32)
+    return sc::set_error(H, SC_EINVAL, "group norm: weight and bias must be in the dtype of x or f32");
+  if (channels < 1 || channels > 4096 || groups < 1 || channels % groups != 0)
+    return sc::set_error(H, SC_EINVAL, "group norm: need 1 <= channels <= 4096, a multiple of groups");
+  if (batch < 1 || !cu) return sc::set_error(H, SC_EINVAL, "group norm: need batch >= 1 and cu_seqlens");
+  if (!offsets_ok(cu, batch))
+    return sc::set_error(H, SC_EINVAL, "group norm: cu_seqlens must start at 0 and be non-decreasing");
+  if (cu[batch] > 0) {
+    if (!x || x_stride < channels) return sc::set_error(H, SC_EINVAL, "group norm: x missing, or x_stride < channels");
+    if (!sc::aligned(x, dtype_bytes(dtype)) || !sc::aligned(weight, dtype_bytes(wdtype)) ||
+        !sc::aligned(bias, dtype_bytes(wdtype)))
+      return sc::set_error(H, SC_EINVAL, "group norm: misaligned pointer");
+  }
+  return SC_OK;
+}
+
+sc_status da_args(Handle* H, const sc_diff_attention_args* a, bool backward, sc::DaArgs* out) {
+  auto bad = [&](const char* what) {
+    return sc::set_error(H, SC_EINVAL, std::string("differential attention: ") + what);
+  };
+  if (a->dtype != SC_BF16 && a->dtype != SC_F16)
+    return sc::set_error(H, SC_EUNSUPPORTED, "differential attention: bf16 or f16 only");
+  if (a->batch < 1 || !a->cu_seqlens_q || !a->cu_seqlens_kv) return bad("need batch >= 1 and both cu_seqlens");
+  if (a->heads < 1 || a->kv_heads < 1 || a->heads % a->kv_heads != 0 || a->heads > 32767)
+    return bad("need 1 <= heads <= 32767, a multiple of kv_heads");
+  if (!offsets_ok(a->cu_seqlens_q, a->batch) || !offsets_ok(a->cu_seqlens_kv, a->batch))
+    return bad("cu_seqlens must start at 0 and be non-decreasing");
+  if (!(a->scale > 0.f) || !(a->scale <= 3.0e38f)) return bad("scale must be positive and finite");
+  if (a->lam) {
+    if (a->lam_count != 1 && a->lam_count != a->heads) return bad("lam_count must be 1 or heads");
+    if (a->lam_dtype != a->dtype && a->lam_dtype != SC_F32) return bad("lam must be in the dtype of q or f32");
+    if (!sc::aligned(a->lam, dtype_bytes(a->lam_dtype))) return bad("misaligned lam");
+  }
+  const int64_t nq = a->cu_seqlens_q[a->batch], nkv = a->cu_seqlens_kv[a->batch];
+  auto row_ok = [](const void* p, int64_t stride, int64_t row) {
+    return p && sc::aligned(p, 16) && stride >= row && stride % 8 == 0;
+  };
+  if (nq > 0 && !row_ok(a->q, a->q_stride, 128ll * a->heads))
+    return bad("q missing, not 16-byte aligned, or a token stride that is short or no multiple of 8");
+  if (nkv > 0 && (!row_ok(a->k, a->k_stride, 128ll * a->kv_heads) || !row_ok(a->v, a->v_stride, 128ll * a->kv_heads)))
+    return bad("k or v missing, not 16-byte aligned, or a token stride that is short or no multiple of 8");
+  if (!backward && nq > 0 && (!a->out || !sc::aligned(a->out, 16))) return bad("out missing or not 16-byte aligned");
+  if (!sc::aligned(a->maps, 16) || !sc::aligned(a->lse, 4)) return bad("misaligned maps or lse");
+  if (nq > 0 && (!a->lse != !a->maps)) return bad("lse and maps go together");
+  if (backward) {
+    if (nq > 0 && (!a->lse || !a->dout || !sc::aligned(a->dout, 16)))
+      return bad("backward needs maps, lse and a 16-byte aligned dout");
+    if (!sc::aligned(a->dq, 16) || !sc::aligned(a->dk, 16) || !sc::aligned(a->dv, 16)) return bad("misaligned gradient");
+    if (a->dlam && (!a->lam || !sc::aligned(a->dlam, dtype_bytes(a->lam_dtype)))) return bad("dlam needs lam");
+  }
+  *out = sc::DaArgs{a->q, a->k, a->v, a->q_stride, a->k_stride, a->v_stride, a->lam, a->lam_count,
+                    static_cast<int>(a->lam_dtype), a->lam_value, a->out, a->lse, a->maps, a->cu_seqlens_q,
+                    a->cu_seqlens_kv, a->batch, a->heads, a->kv_heads, a->scale, a->causal ? 1 : 0, a->dtype, a->dout,
+                    a->dq, a->dk, a->dv, a->dlam};
+  return SC_OK;
+}
+
+}  // namespace
+
+sc_status sc_group_norm(sc_handle* h, const void* x, int64_t x_stride, const void* weight, const void* bias, void* y,
+                        float* stats, const int32_t* cu_seqlens, int32_t batch, int32_t channels, int32_t groups,
+                        float eps, int32_t apply_silu, sc_dtype dtype, sc_dtype wdtype) {
+  if (!h) return SC_EINVAL;
+  Handle* H = &h->impl;
+  const sc_status st = gn_check(H, x, x_stride, weight, bias, cu_seqlens, batch, channels, groups, dtype, wdtype);
+  if (st != SC_OK) return st;
+  if (!(eps > 0.f) || !(eps <= 3.0e38f)) return sc::set_error(H, SC_EINVAL, "group norm: eps must be positive and finite");
+  if (cu_seqlens[batch] == 0) return SC_OK;
+  if (!y || !sc::aligned(y, dtype_bytes(dtype)) || !sc::aligned(stats, 4))
+    return sc::set_error(H, SC_EINVAL, "group norm: y missing, or a misaligned pointer");
+  return guarded(H, [&] {
+    sc::DeviceGuard g(H->device);
+    return sc::group_norm(H, x, x_stride, weight, bias, y, stats, cu_seqlens, batch, channels, groups, eps,
+                          apply_silu ? 1 : 0, dtype, wdtype);
+  });
+}
+
+sc_status sc_group_norm_backward(sc_handle* h, const void* x, int64_t x_stride, const void* dy, const void* weight,
+                                 const void* bias, const float* stats, void* dx, void* dweight, void* dbias,
+                                 const int32_t* cu_seqlens, int32_t batch, int32_t channels, int32_t groups,
+                                 int32_t apply_silu, sc_dtype dtype, sc_dtype wdtype) {
+  if (!h) return SC_EINVAL;
+  Handle* H = &h->impl;
+  const sc_status st = gn_check(H, x, x_stride, weight, bias, cu_seqlens, batch, channels, groups, dtype, wdtype);
+  if (st != SC_OK) return st;
+  if (!dx && !dweight && !dbias) return SC_OK;
+  if (!sc::aligned(dx, dtype_bytes(dtype)) || !sc::aligned(dweight, dtype_bytes(wdtype)) ||
+      !sc::aligned(dbias, dtype_bytes(wdtype)))
+    return sc::set_error(H, SC_EINVAL, "group norm: misaligned pointer");
+  sc::DeviceGuard g(H->device);
+  if (cu_seqlens[batch] == 0) {  // sums over nothing
+    for (void* p : {dweight, dbias})
+      if (p) {
+        const cudaError_t e = cudaMemsetAsync(p, 0, dtype_bytes(wdtype) * channels, H->stream);
+        if (e != cudaSuccess) return sc::cuda_error(H, e, "group norm: zero gradient");
+      }
+    return SC_OK;
+  }
+  if (!dy || !stats || !sc::aligned(dy, dtype_bytes(dtype)) || !sc::aligned(stats, 4))
+    return sc::set_error(H, SC_EINVAL, "group norm: dy or stats missing, or misaligned");
+  return guarded(H, [&] {
+    return sc::group_norm_backward(H, x, x_stride, dy, weight, bias, stats, dx, dweight, dbias, cu_seqlens, batch,
+                                   channels, groups, apply_silu ? 1 : 0, dtype, wdtype);
+  });
+}
+
+sc_status sc_diff_attention(sc_handle* h, const sc_diff_attention_args* args) {
+  if (!h) return SC_EINVAL;
+  Handle* H = &h->impl;
+  if (!args) return sc::set_error(H, SC_EINVAL, "differential attention: null arguments");
+  return guarded(H, [&] {
+    sc::DaArgs a;
+    const sc_status st = da_args(H, args, false, &a);
+    if (st != SC_OK) return st;
+    if (a.cu_q[a.batch] == 0) return SC_OK;
+    sc::DeviceGuard g(H->device);
+    return sc::diff_attention(H, a);
+  });
+}
+
+sc_status sc_diff_attention_backward(sc_handle* h, const sc_diff_attention_args* args) {
+  if (!h) return SC_EINVAL;
+  Handle* H = &h->impl;
+  if (!args) return sc::set_error(H, SC_EINVAL, "differential attention: null arguments");
+  return guarded(H, [&] {
+    sc::DaArgs a;
+    const sc_status st = da_args(H, args, true, &a);
+    if (st != SC_OK) return st;
+    if (!a.dq && !a.dk && !a.dv && !a.dlam) return SC_OK;
+    sc::DeviceGuard g(H->device);
+    return sc::diff_attention_backward(H, a);
+  });
 }
 
 sc_status sc_layernorm_silu(sc_handle* h, void* x, int64_t n, int32_t c, sc_dtype dtype, int32_t apply_silu,

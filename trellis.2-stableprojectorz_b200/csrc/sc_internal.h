@@ -114,6 +114,14 @@ sc_status conv_simt_f32(Handle* h, const KMap* km, const float* feats, const flo
                         const float* residual, float* out, int ci, int co, uint32_t epi, float eps);
 sc_status check_gather_bounds(Handle* h, const KMap* km);
 sc_status layernorm_silu(Handle* h, void* x, int64_t n, int c, sc_dtype dtype, int silu, float eps);
+// group norm over sequences, channels last (sc_groupnorm.cu); cu is a host array
+sc_status group_norm(Handle* h, const void* x, int64_t x_stride, const void* weight, const void* bias, void* y,
+                     float* stats, const int32_t* cu, int batch, int c, int groups, float eps, int silu,
+                     sc_dtype dtype, sc_dtype wdtype);
+sc_status group_norm_backward(Handle* h, const void* x, int64_t x_stride, const void* dy, const void* weight,
+                              const void* bias, const float* stats, void* dx, void* dweight, void* dbias,
+                              const int32_t* cu, int batch, int c, int groups, int silu, sc_dtype dtype,
+                              sc_dtype wdtype);
 // variable-length attention, head dim 64 (sc_attn.cu); cu_q / cu_kv are host arrays
 sc_status attention_varlen(Handle* h, const void* q, const void* k, const void* v, void* out, const int32_t* cu_q,
                            const int32_t* cu_kv, int batch, int heads, float scale, sc_dtype dtype);

@@ -61,6 +61,15 @@ class Engine:
             raise SparseConvError(st, f"sc_create failed on {self.device}")
         self.handle = h
         self.map_mode = map_mode
+        # A second handle for the operators whose backward pass autograd runs
+        # on its own threads: its stream is bound and its calls made under a lock.
+        self._op_lock = threading.Lock()
+        oh = ctypes.c_void_p()
+        st = self.lib.sc_create(ctypes.byref(oh), ctypes.byref(cfg))
+        if st != L.SC_OK:
+            self.close()
+            raise SparseConvError(st, f"sc_create failed on {self.device}")
+        self._op_handle = oh
 
     def bind_stream(self, stream=None):
         s = torch.cuda.current_stream(self.device) if stream is None else stream
@@ -69,21 +78,30 @@ class Engine:
     def check(self, status, what=""):
         L.check(status, self.handle, what)
 
+    def call(self, name, *args):
+        """One library call on torch's current stream of this device, safe from any thread."""
+        with self._op_lock:
+            self.lib.sc_set_stream(self._op_handle, torch.cuda.current_stream(self.device).cuda_stream)
+            L.check(getattr(self.lib, name)(self._op_handle, *args), self._op_handle, name)
+
     def set_conv_ctas(self, max_ctas=0):
         """CTAs of the persistent conv (0 = one per SM); fewer leave SMs for a concurrent collective."""
         self.check(self.lib.sc_set_conv_ctas(self.handle, int(max_ctas)), "sc_set_conv_ctas")
 
     def launch_count(self):
         """Kernels launched through this handle so far."""
-        return int(self.lib.sc_launch_count(self.handle))
+        return int(self.lib.sc_launch_count(self.handle)) + int(self.lib.sc_launch_count(self._op_handle))
 
     def synchronize(self):
         self.check(self.lib.sc_synchronize(self.handle), "synchronize")
+        with self._op_lock:
+            L.check(self.lib.sc_synchronize(self._op_handle), self._op_handle, "synchronize")
 
     def close(self):
-        if getattr(self, "handle", None):
-            self.lib.sc_destroy(self.handle)
-            self.handle = None
+        for name in ("handle", "_op_handle"):
+            if getattr(self, name, None):
+                self.lib.sc_destroy(getattr(self, name))
+                setattr(self, name, None)
 
 
 _engines = {}
