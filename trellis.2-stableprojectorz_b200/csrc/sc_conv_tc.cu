@@ -1111,6 +1111,25 @@ bool make_map_3d(CUtensorMap* m, bool bf16, const void* base, const uint64_t dim
              CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// Tiled map of `rank` <= 5 dimensions, 128-byte swizzle (strides in bytes, of
+// dimensions 1 .. rank - 1).
+bool make_map_nd(CUtensorMap* m, bool bf16, const void* base, int rank, const uint64_t* dims, const uint64_t* strides,
+                 const uint32_t* box) {
+  EncodeTiledFn enc = encode_fn();
+  if (!enc || rank < 1 || rank > 5) return false;
+  cuuint64_t d[5], st[4];
+  cuuint32_t bx[5], estr[5];
+  for (int i = 0; i < rank; ++i) {
+    d[i] = dims[i];
+    bx[i] = box[i];
+    estr[i] = 1;
+    if (i > 0) st[i - 1] = strides[i - 1];
+  }
+  return enc(m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, rank,
+             const_cast<void*>(base), d, st, bx, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+             CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 // Debug mode: verifies every gather index of the map lies in [-1, n_in).
 sc_status check_gather_bounds(Handle* h, const KMap* km) {
   const int64_t total = km->num_tiles * km->K * kTileRows;
