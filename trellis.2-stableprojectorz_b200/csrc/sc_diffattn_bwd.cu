@@ -7,6 +7,23 @@
 //   dlam_h = -sum_rows delta_2,
 // dK and dV summed over the heads that share a key / value head.  O_1 and O_2
 // are kept by the forward in f32.  Every sum has one fixed order.
+//
+// Two kernels of one shape (k_da_bwd): a CTA holds 128 rows X (queries for dQ,
+// keys for dK and dV) and walks 64-row tiles of the other side Y.  Both maps
+// share dP, and dV takes one product with the combined weights, so a pair of
+// rows costs 768 flops in the dQ kernel and 1024 in the other.  Accumulating
+// dQ in the dK / dV kernel instead would save the second recomputation, but
+// needs sums across CTAs whose order changes from run to run.
+//   warp 0     TMA producer: X's Q / K pair and its dO / V once, then Y's 32 KB
+//              (and, for keys, the 64 rows' statistics) into a ring of four
+//   warp 1     issues S_m = X_m Y_m^T and dP (128 x 64 each) into tensor
+//              memory, and the accumulations dX_m += dS_m Y_m, dV += P dO with
+//              dS and P as A operands in tensor memory, Y MN-major
+//   warp 2     zeroes Y rows behind the last visible one (0 * NaN)
+//   warps 4-11 the elementwise part, one row per lane, columns 0-31 / 32-63
+// S of the next tile is issued as soon as the weights of this one are in
+// registers, so the exponentials overlap the accumulations.
+// Every mbarrier wait is bounded (SC_ETIMEOUT).
 #include "sc_diffattn_dev.cuh"
 
 #include <algorithm>
@@ -15,18 +32,32 @@
 namespace sc {
 namespace {
 
+constexpr int kX = 128;                   // rows per CTA
+constexpr int kY = 64;                    // rows per step
+constexpr int kStages = 4;
+constexpr int kThreads = 384;
+constexpr int kXBytes = kX * kDaD * 2;    // 16 KB
+constexpr int kYBytes = kY * kDaD * 2;    // 8 KB
+constexpr int kStageBytes = 4 * kYBytes + 4 * kY * 4;  // Y_1, Y_2, halves of the 128-wide one, statistics
+constexpr int kOffX = 0;                  // X_1, X_2, halves of the 128-wide one
+constexpr int kOffY = 4 * kXBytes;
+constexpr int kOffBar = kOffY + kStages * kStageBytes;
+constexpr int kSmem = kOffBar + 256 + 1024;
+// tensor memory columns
+constexpr uint32_t kTmem = 512, kColS = 0, kColDp = 128, kColP = 192, kColDs1 = 224, kColX = 256, kColV = 384;
+
 struct DaBwd {
-  const void *q, *k, *v;
-  int64_t qs, ks, vs;
   LamRef lam;
+  const float* lse;    // [2][heads][nq]
   const float* maps;   // [nq][heads][2][128]
   const void* dout;
-  const float* lse;    // [2][heads][nq]
-  float* delta;        // [2][heads][nq]
+  float* st;           // [4][heads][np]: -lse_1, -lse_2, -delta_1, -delta_2
+  int64_t np;          // rows of st: sequences start at multiples of 4
   void *dq, *dk, *dv, *dlam;
   int64_t nq;
   int heads, kv_heads, rep, causal;
   float scale, scale_log2;
+  int* err;
 };
 
 __device__ __forceinline__ float warp_add(float v) {
@@ -34,42 +65,60 @@ __device__ __forceinline__ float warp_add(float v) {
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
+__device__ __forceinline__ unsigned long long mul_f2(unsigned long long a, unsigned long long b) {
+  unsigned long long d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+// Stores 16 consecutive 32-bit columns of this thread's TMEM lane.
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&v)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+      "%15, %16};" ::"r"(taddr),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+      "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+      : "memory");
+}
 
-// delta_1, delta_2 of every (row, head), one warp each.
+// Statistics of every (row, head), one warp each.  Records: aux = the
+// sequence's first row in st.
 template <typename T>
-__global__ void __launch_bounds__(256) k_da_delta(const DaBwd p) {
+__global__ void __launch_bounds__(256) k_da_stats(const DaBwd p, const __grid_constant__ SeqPlan plan) {
   const int64_t at = blockIdx.x * 8ll + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
   if (at >= p.nq * p.heads) return;
-  const int64_t row = at / p.heads;
-  const int h = static_cast<int>(at % p.heads);
+  const int row = static_cast<int>(at / p.heads), h = static_cast<int>(at % p.heads);
+  const SeqRec& r = plan.at(plan.find(row));
   const float4 o1 = reinterpret_cast<const float4*>(p.maps + at * 2 * kDaDv)[lane];
   const float4 o2 = reinterpret_cast<const float4*>(p.maps + at * 2 * kDaDv + kDaDv)[lane];
   const uint2 raw = reinterpret_cast<const uint2*>(static_cast<const T*>(p.dout) + at * kDaDv)[lane];
   const T* g = reinterpret_cast<const T*>(&raw);
   const float g0 = Cvt<T>::to_f(g[0]), g1 = Cvt<T>::to_f(g[1]), g2 = Cvt<T>::to_f(g[2]), g3 = Cvt<T>::to_f(g[3]);
-  float d1 = fmaf(g0, o1.x, g1 * o1.y) + fmaf(g2, o1.z, g3 * o1.w);
-  float d2 = fmaf(g0, o2.x, g1 * o2.y) + fmaf(g2, o2.z, g3 * o2.w);
-  d1 = warp_add(d1);
-  d2 = warp_add(d2);
-  if (lane == 0) {
-    p.delta[h * p.nq + row] = d1;
-    p.delta[(p.heads + h) * p.nq + row] = d2;
+  const float d1 = warp_add(fmaf(g0, o1.x, g1 * o1.y) + fmaf(g2, o1.z, g3 * o1.w));
+  const float d2 = warp_add(fmaf(g0, o2.x, g1 * o2.y) + fmaf(g2, o2.z, g3 * o2.w));
+  if (lane < 4) {
+    const float v = lane < 2 ? p.lse[(static_cast<int64_t>(lane) * p.heads + h) * p.nq + row] : lane == 2 ? d1 : d2;
+    float* dst = p.st + (static_cast<int64_t>(lane) * p.heads + h) * p.np + r.aux + (row - r.q0);
+    dst[0] = -v;
+    if (row == r.q1 - 1)  // up to three rows between sequences
+      for (int i = 1; (r.aux + row - r.q0 + i) & 3; ++i) dst[i] = 0.f;
   }
 }
 
 // dlam: one CTA per entry of lam sums -delta_2 over its heads' rows.
-__global__ void __launch_bounds__(1024) k_da_dlam(const DaBwd p) {
+__global__ void __launch_bounds__(1024) k_da_dlam(const DaBwd p, int64_t rows) {
   __shared__ float s[32];
-  const int64_t n = p.lam.count == 1 ? p.nq * p.heads : p.nq;
-  const float* d = p.delta + p.heads * p.nq + blockIdx.x * p.nq;
+  const int heads = p.lam.count == 1 ? p.heads : 1;
   float a = 0.f;
-  for (int64_t i = threadIdx.x; i < n; i += 1024) a += d[i];
+  for (int k = 0; k < heads; ++k) {
+    const float* d = p.st + (3ll * p.heads + blockIdx.x + k) * p.np;
+    for (int64_t i = threadIdx.x; i < rows; i += 1024) a += d[i];
+  }
   a = warp_add(a);
   if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = a;
   __syncthreads();
   if (threadIdx.x < 32) {
-    a = -warp_add(s[threadIdx.x]);
+    a = warp_add(s[threadIdx.x]);
     if (threadIdx.x == 0) {
       if (p.lam.dtype == SC_F32) static_cast<float*>(p.dlam)[blockIdx.x] = a;
       else if (p.lam.dtype == SC_BF16) static_cast<__nv_bfloat16*>(p.dlam)[blockIdx.x] = __float2bfloat16_rn(a);
@@ -78,151 +127,469 @@ __global__ void __launch_bounds__(1024) k_da_dlam(const DaBwd p) {
   }
 }
 
-// p_1, p_2, ds_1, ds_2 of one (query, key) pair, each product over one lane's dims.
-template <typename T>
-__device__ __forceinline__ void pair(const DaBwd& p, const T* q, const T* k, const T* v, const T* g, int h,
-                                     int64_t row, float lam, float (&pm)[2], float (&ds)[2]) {
-  float dp = 0.f;
-  for (int e = 0; e < kDaDv; ++e) dp = fmaf(Cvt<T>::to_f(g[e]), Cvt<T>::to_f(v[e]), dp);
-#pragma unroll
-  for (int s = 0; s < 2; ++s) {
-    float d = 0.f;
-    for (int e = 0; e < kDaD; ++e) d = fmaf(Cvt<T>::to_f(q[s * kDaD + e]), Cvt<T>::to_f(k[s * kDaD + e]), d);
-    const int64_t at = (static_cast<int64_t>(s) * p.heads + h) * p.nq + row;
-    pm[s] = exp2f(fmaf(d, p.scale_log2, -p.lse[at]));
-    ds[s] = (s ? -lam : 1.f) * pm[s] * (dp - p.delta[at]);
-  }
-}
+// KV false: X = queries of one head, Y = keys; writes dQ.  KV true: X = keys of
+// one key / value head, Y = the queries of each of its heads in turn; writes
+// dK and dV.  tmX / tmXw: the 64- and 128-wide rows of X in boxes of 128; tmY /
+// tmYw likewise in boxes of 64.  Records: item0 counts tiles of X, aux = the
+// sequence's first row in st.
+template <typename T, bool KV>
+__global__ void __launch_bounds__(kThreads, 1)
+    k_da_bwd(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmXw,
+             const __grid_constant__ CUtensorMap tmY, const __grid_constant__ CUtensorMap tmYw, const DaBwd p,
+             const __grid_constant__ SeqPlan plan) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const uint32_t sbase = smem_u32(smem);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kOffBar);
+  uint32_t* s_tmem = reinterpret_cast<uint32_t*>(bars + 24);
+  const uint32_t x_full = smem_u32(bars);
+  const uint32_t y_full0 = x_full + 8, y_empty0 = y_full0 + 8 * kStages;
+  const uint32_t s_full = y_empty0 + 8 * kStages;  // S_1, S_2 written
+  const uint32_t s_free = s_full + 8;              // S_1, S_2 read
+  const uint32_t dp_full = s_free + 8, dp_free = dp_full + 8;  // dP written; dX_2's product (over dP's columns) done
+  const uint32_t ds_full = dp_free + 8;            // P, dS_1, dS_2 written
+  const uint32_t p_free = ds_full + 8;             // their products done
+  const uint32_t y_req = p_free + 8, y_fixed = y_req + 8, done_bar = y_fixed + 8;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const SeqRec& rec = plan.at(plan.find(blockIdx.x));
+  const int lq = rec.q1 - rec.q0, lk = rec.k1 - rec.k0;
+  const int ntiles = ((KV ? lk : lq) + kX - 1) / kX;
+  int xt = blockIdx.x - rec.item0;
+  if (!KV) xt = ntiles - 1 - xt;  // causal: the longest first
+  const int x0 = xt * kX, nx = min(kX, (KV ? lk : lq) - x0);
+  const int g = KV ? blockIdx.y : blockIdx.y / p.rep;
+  // rows [y0, y1) of Y in steps of 64, for each of nh heads
+  const int y1 = KV ? lq : key_limit(rec, x0 + nx - 1, p.causal);
+  const int y0 = KV && p.causal ? max(0, x0 - lk + lq) / kY * kY : 0;
+  const int ny = y1 > y0 ? (y1 - y0 + kY - 1) / kY : 0;
+  const int nh = KV ? p.rep : 1, n = ny * nh;
+  const bool last_partial = (y1 - y0) % kY != 0;
 
-template <typename T>
-__global__ void __launch_bounds__(128) k_da_dq_rows(const DaBwd p, const __grid_constant__ SeqPlan plan, int items) {
-  const int item = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31, h = blockIdx.y;
-  if (item >= items) return;
-  const SeqRec& r = plan.at(plan.find(item));
-  const int i = item - r.item0, limit = key_limit(r, i, p.causal), g = h / p.rep;
-  const int64_t row = r.q0 + i;
-  const T* q = static_cast<const T*>(p.q) + row * p.qs + 2 * h * kDaD;
-  const T* go = static_cast<const T*>(p.dout) + (row * p.heads + h) * kDaDv;
-  const float lam = p.lam.get(h);
-  float acc[2][2] = {};
-  for (int j0 = 0; j0 < limit; j0 += 32) {
-    const int64_t j = r.k0 + static_cast<int64_t>(min(j0 + lane, limit - 1));
-    float pm[2], ds[2];
-    pair<T>(p, q, static_cast<const T*>(p.k) + j * p.ks + 2 * g * kDaD, static_cast<const T*>(p.v) + j * p.vs + g * kDaDv,
-            go, h, row, lam, pm, ds);
-    for (int t = 0; t < min(32, limit - j0); ++t) {
-      const T* k = static_cast<const T*>(p.k) + (r.k0 + static_cast<int64_t>(j0 + t)) * p.ks + 2 * g * kDaD + 2 * lane;
-#pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        const float d = __shfl_sync(0xffffffffu, ds[s], t);
-#pragma unroll
-        for (int e = 0; e < 2; ++e) acc[s][e] = fmaf(d, Cvt<T>::to_f(k[s * kDaD + e]), acc[s][e]);
+  if (threadIdx.x == 0) {
+    mbar_init(x_full, 1);
+    for (int st = 0; st < kStages; ++st) {
+      mbar_init(y_full0 + 8 * st, 1);
+      mbar_init(y_empty0 + 8 * st, 1);
+    }
+    mbar_init(s_full, 1);
+    mbar_init(s_free, 8);
+    mbar_init(dp_full, 1);
+    mbar_init(dp_free, 1);
+    mbar_init(ds_full, 8);
+    mbar_init(p_free, 1);
+    mbar_init(y_req, 1);
+    mbar_init(y_fixed, 1);
+    mbar_init(done_bar, 1);
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(smem_u32(s_tmem), kTmem);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *s_tmem;
+
+  if (warp == 0) {
+    // ----------------------------------------------------------- producer
+    if (lane == 0 && n > 0) {
+      const int xrow = (KV ? rec.k0 : rec.q0) + x0, xh = blockIdx.y;
+      mbar_arrive_expect_tx(x_full, 4 * kXBytes);
+      tma_load_3d(sbase + kOffX, &tmX, 0, 2 * xh, xrow, x_full);
+      tma_load_3d(sbase + kOffX + kXBytes, &tmX, 0, 2 * xh + 1, xrow, x_full);
+      tma_load_3d(sbase + kOffX + 2 * kXBytes, &tmXw, 0, xh, xrow, x_full);
+      tma_load_3d(sbase + kOffX + 3 * kXBytes, &tmXw, 64, xh, xrow, x_full);
+      for (int j = 0; j < n; ++j) {
+        const int st = j % kStages;
+        if (!mbar_wait(y_empty0 + 8 * st, ((j / kStages) & 1) ^ 1, p.err)) break;
+        const uint32_t yb = sbase + kOffY + st * kStageBytes, bar = y_full0 + 8 * st;
+        const int yh = KV ? g * p.rep + j / ny : g, yr = y0 + (j % ny) * kY, yrow = (KV ? rec.q0 : rec.k0) + yr;
+        mbar_arrive_expect_tx(bar, 4 * kYBytes + (KV ? 4 * kY * 4 : 0));
+        tma_load_3d(yb, &tmY, 0, 2 * yh, yrow, bar);
+        tma_load_3d(yb + kYBytes, &tmY, 0, 2 * yh + 1, yrow, bar);
+        tma_load_3d(yb + 2 * kYBytes, &tmYw, 0, yh, yrow, bar);
+        tma_load_3d(yb + 3 * kYBytes, &tmYw, 64, yh, yrow, bar);
+        if (KV)  // st rows start at multiples of 4: 16-byte aligned, and st has 64 rows behind its last
+          for (int k = 0; k < 4; ++k)
+            bulk_load(yb + 4 * kYBytes + k * kY * 4, p.st + (static_cast<int64_t>(k) * p.heads + yh) * p.np + rec.aux + yr,
+                      kY * 4, bar);
       }
     }
-  }
-  T* dq = static_cast<T*>(p.dq) + (row * 2 * p.heads + 2 * h) * kDaD + 2 * lane;
+  } else if (warp == 1) {
+    // ---------------------------------------------------------- MMA issuer
+    if (lane == 0 && n > 0) {
+      const bool bf16 = std::is_same_v<T, __nv_bfloat16>;
+      const uint32_t id_s = idesc_f16(128, 64, bf16), id_x = id_s | (1u << 16),
+                     id_v = idesc_f16(128, 128, bf16) | (1u << 16);
+      auto ybase = [&](int j) { return sbase + kOffY + (j % kStages) * kStageBytes; };
+      auto issue_s = [&](int j) {
 #pragma unroll
-  for (int s = 0; s < 2; ++s)
+        for (int m = 0; m < 2; ++m)
 #pragma unroll
-    for (int e = 0; e < 2; ++e) dq[s * kDaD + e] = Cvt<T>::from_f(acc[s][e] * p.scale);
-}
-
-template <typename T>
-__global__ void __launch_bounds__(128) k_da_dkv_rows(const DaBwd p, const __grid_constant__ SeqPlan plan, int items) {
-  const int item = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31, g = blockIdx.y;
-  if (item >= items) return;
-  const SeqRec& r = plan.at(plan.find(item));
-  const int j = item - r.item0, lq = r.q1 - r.q0;
-  const int64_t row = r.k0 + j;
-  const T* k = static_cast<const T*>(p.k) + row * p.ks + 2 * g * kDaD;
-  const T* v = static_cast<const T*>(p.v) + row * p.vs + g * kDaDv;
-  const int first = p.causal ? min(lq, max(0, j - (r.k1 - r.k0) + lq)) : 0;  // first query that sees key j
-  float ak[2][2] = {}, av[4] = {};
-  for (int h = g * p.rep; h < (g + 1) * p.rep; ++h) {
-    const float lam = p.lam.get(h);
-    for (int i0 = first; i0 < lq; i0 += 32) {
-      const int64_t i = r.q0 + static_cast<int64_t>(min(i0 + lane, lq - 1));
-      float pm[2], ds[2];
-      pair<T>(p, static_cast<const T*>(p.q) + i * p.qs + 2 * h * kDaD, k, v,
-              static_cast<const T*>(p.dout) + (i * p.heads + h) * kDaDv, h, i, lam, pm, ds);
-      const float pd = fmaf(-lam, pm[1], pm[0]);
-      for (int t = 0; t < min(32, lq - i0); ++t) {
-        const int64_t it = r.q0 + static_cast<int64_t>(i0 + t);
-        const T* q = static_cast<const T*>(p.q) + it * p.qs + 2 * h * kDaD + 2 * lane;
-        const T* go = static_cast<const T*>(p.dout) + (it * p.heads + h) * kDaDv + 4 * lane;
+          for (int k = 0; k < kDaD / 16; ++k)
+            tc_mma_f16(tmem + kColS + 64u * m, smem_desc(sbase + kOffX + m * kXBytes + 32u * k, 1024, 2),
+                       smem_desc(ybase(j) + m * kYBytes + 32u * k, 1024, 2), id_s, k > 0 ? 1u : 0u);
+        tc_commit(s_full);
+      };
+      auto issue_dp = [&](int j) {
 #pragma unroll
-        for (int s = 0; s < 2; ++s) {
-          const float d = __shfl_sync(0xffffffffu, ds[s], t);
-#pragma unroll
-          for (int e = 0; e < 2; ++e) ak[s][e] = fmaf(d, Cvt<T>::to_f(q[s * kDaD + e]), ak[s][e]);
+        for (int k = 0; k < kDaDv / 16; ++k)
+          tc_mma_f16(tmem + kColDp, smem_desc(sbase + kOffX + (2 + k / 4) * kXBytes + 32u * (k % 4), 1024, 2),
+                     smem_desc(ybase(j) + (2 + k / 4) * kYBytes + 32u * (k % 4), 1024, 2), id_s, k > 0 ? 1u : 0u);
+        tc_commit(dp_full);
+      };
+      auto landed = [&](int j) {
+        const bool r = mbar_wait(y_full0 + 8 * (j % kStages), (j / kStages) & 1, p.err);
+        if (r && last_partial && j % ny == ny - 1) mbar_arrive(y_req);
+        return r;
+      };
+      bool ok = mbar_wait(x_full, 0, p.err) && landed(0);
+      if (ok) {
+        tc_fence_after();
+        issue_s(0);
+        issue_dp(0);
+      }
+      for (int j = 0; ok && j < n; ++j) {
+        const bool more = j + 1 < n;
+        const bool partial = last_partial && j % ny == ny - 1;
+        // the zeroed rows of step j first: y_req of a later step waits for them
+        if (partial) ok = mbar_wait(y_fixed, (j / ny) & 1, p.err);
+        if (ok && more) {
+          ok = landed(j + 1) && mbar_wait(s_free, j & 1, p.err);
+          if (!ok) break;
+          tc_fence_after();
+          issue_s(j + 1);
         }
-        const float d = __shfl_sync(0xffffffffu, pd, t);
+        ok = ok && mbar_wait(ds_full, j & 1, p.err);
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t acc = j > 0 ? 1u : 0u;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) av[e] = fmaf(d, Cvt<T>::to_f(go[e]), av[e]);
+        for (int k = 0; k < kY / 16; ++k)  // dS_2 lies over the halves of dP that its warps read
+          tc_mma_f16_tmem_a(tmem + kColX + 64u, tmem + kColDp + 32u * (k / 2) + 8u * (k % 2),
+                            smem_desc_mn(ybase(j) + kYBytes + 2048u * k, kYBytes), id_x, k > 0 ? 1u : acc);
+        tc_commit(dp_free);
+#pragma unroll
+        for (int k = 0; k < kY / 16; ++k)
+          tc_mma_f16_tmem_a(tmem + kColX, tmem + kColDs1 + 8u * k, smem_desc_mn(ybase(j) + 2048u * k, kYBytes), id_x,
+                            k > 0 ? 1u : acc);
+        if (KV) {
+#pragma unroll
+          for (int k = 0; k < kY / 16; ++k)
+            tc_mma_f16_tmem_a(tmem + kColV, tmem + kColP + 8u * k,
+                              smem_desc_mn(ybase(j) + 2 * kYBytes + 2048u * k, kYBytes), id_v, k > 0 ? 1u : acc);
+        }
+        tc_commit(p_free);
+        tc_commit(y_empty0 + 8 * (j % kStages));
+        if (more) {
+          ok = mbar_wait(dp_free, j & 1, p.err);
+          if (!ok) break;
+          tc_fence_after();
+          issue_dp(j + 1);
+        }
+      }
+      tc_commit(done_bar);  // every product ends before its tensor memory is released
+      mbar_wait(done_bar, 0, p.err);
+    }
+  } else if (warp == 2) {
+    // ------------------------------------------ Y rows behind the last visible one
+    if (last_partial && n > 0) {
+      const uint32_t valid = (y1 - y0) - (ny - 1) * kY;
+      for (int hh = 0; hh < nh; ++hh) {
+        int w = 1;
+        if (lane == 0) w = mbar_wait(y_req, hh & 1, p.err) ? 1 : 0;
+        if (__shfl_sync(0xffffffffu, w, 0) == 0) break;
+        const uint32_t yb = sbase + kOffY + ((hh * ny + ny - 1) % kStages) * kStageBytes;
+        for (uint32_t a = 128u * valid + 16u * lane; a < static_cast<uint32_t>(kYBytes); a += 512u)
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(yb + k * kYBytes + a), "r"(0u) : "memory");
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(y_fixed);
+      }
+    }
+  } else if (warp >= 4) {
+    // ------------------------------------------------- weights and score gradients
+    const int hf = (warp - 4) >> 2, row = (warp & 3) * 32 + lane, x = x0 + row;  // x: row of the sequence
+    const uint32_t lane_base = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+    const bool live = row < nx;
+    // this row sees the Y rows [lo, hi)
+    const int lo = KV && p.causal ? x - lk + lq : 0;
+    const int hi = KV ? lq : (live ? key_limit(rec, x, p.causal) : y1);
+    const int lo_max = __reduce_max_sync(0xffffffffu, lo), hi_min = __reduce_min_sync(0xffffffffu, hi);
+    float nl[2] = {0.f, 0.f}, nd[2] = {0.f, 0.f};
+    if (!KV && live)
+#pragma unroll
+      for (int m = 0; m < 2; ++m) {
+        const int64_t at = static_cast<int64_t>(blockIdx.y) * p.np + rec.aux + x;
+        nl[m] = p.st[m * static_cast<int64_t>(p.heads) * p.np + at];
+        nd[m] = p.st[(2 + m) * static_cast<int64_t>(p.heads) * p.np + at];
+      }
+    bool ok = true;
+    auto wait_warp = [&](uint32_t bar, uint32_t parity) -> bool {
+      int w = 1;
+      if (lane == 0) w = mbar_wait(bar, parity, p.err) ? 1 : 0;
+      return __shfl_sync(0xffffffffu, w, 0) != 0;
+    };
+    const unsigned long long sc2 = f2(p.scale_log2, p.scale_log2);
+    for (int j = 0; j < n; ++j) {
+      const int c0 = y0 + (j % ny) * kY + 32 * hf;  // first of this thread's 32 columns
+      const bool full = c0 >= lo_max && c0 + 32 <= hi_min;
+      const float nlam = -p.lam.get(KV ? g * p.rep + j / ny : blockIdx.y);
+      const float4* st = reinterpret_cast<const float4*>(smem + kOffY + (j % kStages) * kStageBytes + 4 * kYBytes) + 8 * hf;
+      if (!wait_warp(s_full, j & 1)) {
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      // statistics of Y land with its tile: the MMA thread has seen them, this thread has not
+      if (KV && !wait_warp(y_full0 + 8 * (j % kStages), (j / kStages) & 1)) {
+        ok = false;
+        break;
+      }
+      float w[2][32];
+#pragma unroll
+      for (int m = 0; m < 2; ++m) {
+        float s[32];
+        tmem_ld32(lane_base + kColS + 64u * m + 32u * hf, s);
+#pragma unroll
+        for (int i = 0; i < 32; i += 4) {
+          float4 l4;
+          if (KV) l4 = st[16 * m + i / 4];
+          else l4 = make_float4(nl[m], nl[m], nl[m], nl[m]);
+          float a, b, c, d;
+          f2_split(fma_f2(f2(s[i], s[i + 1]), sc2, f2(l4.x, l4.y)), a, b);
+          f2_split(fma_f2(f2(s[i + 2], s[i + 3]), sc2, f2(l4.z, l4.w)), c, d);
+          w[m][i] = ex2_ftz(a);
+          w[m][i + 1] = ex2_ftz(b);
+          w[m][i + 2] = ex2_ftz(c);
+          w[m][i + 3] = ex2_ftz(d);
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(s_free);
+      if (!full) {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          const bool see = c0 + i >= lo && c0 + i < hi;
+          w[0][i] = see ? w[0][i] : 0.f;
+          w[1][i] = see ? w[1][i] : 0.f;
+        }
+      }
+      if (!wait_warp(dp_full, j & 1)) {
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      float dp[32];
+      tmem_ld32(lane_base + kColDp + 32u * hf, dp);
+      if (!full) {  // 0 * NaN of a row that is not seen
+#pragma unroll
+        for (int i = 0; i < 32; ++i) dp[i] = (c0 + i >= lo && c0 + i < hi) ? dp[i] : 0.f;
+      }
+      uint32_t pk[16], k1[16], k2[16];
+      const unsigned long long nlam2 = f2(nlam, nlam);
+#pragma unroll
+      for (int i = 0; i < 32; i += 4) {
+        float4 d1, d2;
+        if (KV) {
+          d1 = st[32 + i / 4];
+          d2 = st[48 + i / 4];
+          if (!full) {
+            float* e1 = &d1.x;
+            float* e2 = &d2.x;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const bool see = c0 + i + k >= lo && c0 + i + k < hi;
+              e1[k] = see ? e1[k] : 0.f;
+              e2[k] = see ? e2[k] : 0.f;
+            }
+          }
+        } else {
+          d1 = make_float4(nd[0], nd[0], nd[0], nd[0]);
+          d2 = make_float4(nd[1], nd[1], nd[1], nd[1]);
+        }
+#pragma unroll
+        for (int k = 0; k < 4; k += 2) {
+          const unsigned long long dd = f2(dp[i + k], dp[i + k + 1]);
+          const unsigned long long w1 = f2(w[0][i + k], w[0][i + k + 1]);
+          const unsigned long long w2 = mul_f2(nlam2, f2(w[1][i + k], w[1][i + k + 1]));  // -lam P_2
+          float a, b;
+          f2_split(mul_f2(w1, add_f2(dd, k ? f2(d1.z, d1.w) : f2(d1.x, d1.y))), a, b);
+          k1[(i + k) / 2] = pack2<T>(a, b);
+          f2_split(mul_f2(w2, add_f2(dd, k ? f2(d2.z, d2.w) : f2(d2.x, d2.y))), a, b);
+          k2[(i + k) / 2] = pack2<T>(a, b);
+          if (KV) {
+            f2_split(add_f2(w1, w2), a, b);
+            pk[(i + k) / 2] = pack2<T>(a, b);
+          }
+        }
+      }
+      if (j > 0 && !wait_warp(p_free, (j - 1) & 1)) {
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      if (KV) tmem_st16(lane_base + kColP + 16u * hf, pk);
+      tmem_st16(lane_base + kColDs1 + 16u * hf, k1);
+      tmem_st16(lane_base + kColDp + 32u * hf, k2);
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(ds_full);
+    }
+    ok = ok && n > 0 && wait_warp(p_free, (n - 1) & 1);
+    tc_fence_after();
+    // group hf writes dX_(hf+1), and half hf of dV's columns
+    const int64_t xr = static_cast<int64_t>(KV ? rec.k0 : rec.q0) + x;
+    const int xheads = KV ? p.kv_heads : p.heads;
+    T* dx = static_cast<T*>(KV ? p.dk : p.dq);
+    T* dv = static_cast<T*>(p.dv);
+#pragma unroll
+    for (int part = 0; part < (KV ? 2 : 1); ++part) {
+      T* base = part ? dv : dx;
+      if (!base) continue;  // uniform over the grid
+      const float mul = part ? 1.f : p.scale;
+      T* dst = base + (part ? (xr * xheads + blockIdx.y) * kDaDv + 64 * hf
+                            : (xr * xheads + blockIdx.y) * (2 * kDaD) + kDaD * hf);
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        float o[32];
+        __syncwarp();
+        if (n > 0) tmem_ld32(lane_base + (part ? kColV : kColX) + 64u * hf + 32u * c, o);
+        if (live) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            uint32_t u[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              u[k] = ok ? pack2<T>(o[8 * i + 2 * k] * mul, o[8 * i + 2 * k + 1] * mul) : 0u;
+            reinterpret_cast<uint4*>(dst + 32 * c)[i] = make_uint4(u[0], u[1], u[2], u[3]);
+          }
+        }
       }
     }
   }
-  if (p.dk) {
-    T* dk = static_cast<T*>(p.dk) + (row * 2 * p.kv_heads + 2 * g) * kDaD + 2 * lane;
-#pragma unroll
-    for (int s = 0; s < 2; ++s)
-#pragma unroll
-      for (int e = 0; e < 2; ++e) dk[s * kDaD + e] = Cvt<T>::from_f(ak[s][e] * p.scale);
-  }
-  if (p.dv) {
-    T* dv = static_cast<T*>(p.dv) + (row * p.kv_heads + g) * kDaDv + 4 * lane;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) dv[e] = Cvt<T>::from_f(av[e]);
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, kTmem);
   }
 }
 
-// Records of the sequences with rows on the chosen side, one item per row.
-int32_t row_items(const DaArgs& a, bool keys, std::vector<SeqRec>* recs) {
-  int32_t items = 0;
-  const int32_t* cu = keys ? a.cu_kv : a.cu_q;
-  for (int b = 0; b < a.batch; ++b) {
-    if (cu[b + 1] == cu[b]) continue;
-    recs->push_back(SeqRec{a.cu_q[b], a.cu_q[b + 1], a.cu_kv[b], a.cu_kv[b + 1], items, b});
-    items += cu[b + 1] - cu[b];
+bool box_map(CUtensorMap* m, bool bf16, const void* base, int width, int heads, int64_t rows, int64_t stride,
+             int box_rows) {
+  const uint64_t d[3] = {static_cast<uint64_t>(width), static_cast<uint64_t>(heads),
+                         static_cast<uint64_t>(std::max<int64_t>(rows, 1))};
+  const uint64_t s[2] = {static_cast<uint64_t>(width) * 2, static_cast<uint64_t>(stride) * 2};
+  const uint32_t b[3] = {64, 1, static_cast<uint32_t>(box_rows)};
+  return make_map_nd(m, bf16, base, 3, d, s, b);
+}
+
+template <typename T, bool KV>
+sc_status launch_bwd(Handle* h, const DaArgs& a, const DaBwd& p, const std::vector<int32_t>& st_row) {
+  const bool bf16 = std::is_same_v<T, __nv_bfloat16>;
+  const int64_t nq = a.cu_q[a.batch], nkv = a.cu_kv[a.batch];
+  std::vector<SeqRec> recs;
+  for (int b = 0; b < a.batch; ++b)
+    if (KV ? a.cu_kv[b + 1] > a.cu_kv[b] : a.cu_q[b + 1] > a.cu_q[b])
+      recs.push_back(SeqRec{a.cu_q[b], a.cu_q[b + 1], a.cu_kv[b], a.cu_kv[b + 1], 0, st_row[b]});
+  if (recs.empty()) return SC_OK;
+  // the longest walks first: the tail of the launch is made of short CTAs
+  std::stable_sort(recs.begin(), recs.end(), [](const SeqRec& x, const SeqRec& y) {
+    return KV ? x.q1 - x.q0 > y.q1 - y.q0 : x.k1 - x.k0 > y.k1 - y.k0;
+  });
+  int64_t items = 0;
+  for (SeqRec& r : recs) {
+    r.item0 = static_cast<int32_t>(items);
+    items += ((KV ? r.k1 - r.k0 : r.q1 - r.q0) + kX - 1) / kX;
   }
-  return items;
+  // a side without rows is never read, but its maps want an address
+  const void* some = nq > 0 ? a.q : a.k;
+  const void *q = nq > 0 ? a.q : some, *go = nq > 0 ? a.dout : some, *k = nkv > 0 ? a.k : some,
+             *v = nkv > 0 ? a.v : some;
+  const int64_t dense = 128ll * a.heads;
+  const int64_t qs = nq > 0 ? a.qs : dense, ks = nkv > 0 ? a.ks : 128ll * a.kv_heads,
+                vs = nkv > 0 ? a.vs : 128ll * a.kv_heads;
+  CUtensorMap mq, mo, mk, mv;
+  if (!box_map(&mq, bf16, q, kDaD, 2 * a.heads, nq, qs, KV ? kY : kX) ||
+      !box_map(&mo, bf16, go, kDaDv, a.heads, nq, dense, KV ? kY : kX) ||
+      !box_map(&mk, bf16, k, kDaD, 2 * a.kv_heads, nkv, ks, KV ? kX : kY) ||
+      !box_map(&mv, bf16, v, kDaDv, a.kv_heads, nkv, vs, KV ? kX : kY))
+    return set_error(h, SC_ECUDA, "cuTensorMapEncodeTiled failed (differential attention backward)");
+  SeqPlan plan;
+  void* table = nullptr;
+  const sc_status st = make_plan(h, recs, &plan, &table);
+  if (st != SC_OK) return st;
+  cudaError_t e = cudaFuncSetAttribute(k_da_bwd<T, KV>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+  if (e == cudaSuccess) {
+    ++h->launches;
+    const dim3 grid(static_cast<unsigned>(items), KV ? a.kv_heads : a.heads);
+    if (KV) k_da_bwd<T, KV><<<grid, kThreads, kSmem, h->stream>>>(mk, mv, mq, mo, p, plan);
+    else k_da_bwd<T, KV><<<grid, kThreads, kSmem, h->stream>>>(mq, mo, mk, mv, p, plan);
+    e = cudaGetLastError();
+  }
+  dev_free(h, table);
+  return e == cudaSuccess ? SC_OK : cuda_error(h, e, "differential attention backward launch");
 }
 
 template <typename T>
 sc_status run_backward(Handle* h, const DaArgs& a) {
   const int64_t nq = a.cu_q[a.batch];
-  DaBwd p{a.q, a.k, a.v, a.qs, a.ks, a.vs, LamRef{a.lam, a.lam_count, a.lam_dtype, a.lam_value}, a.maps, a.dout, a.lse,
-          nullptr, a.dq, a.dk, a.dv, a.dlam, nq, a.heads, a.kv_heads, a.heads / a.kv_heads, a.causal, a.scale,
-          a.scale * kLog2e};
-  void* tables[2] = {nullptr, nullptr};
-  cudaError_t e = dev_alloc(h, reinterpret_cast<void**>(&p.delta), sizeof(float) * 2 * a.heads * nq);
+  DaBwd p{};
+  p.lam = LamRef{a.lam, a.lam_count, a.lam_dtype, a.lam_value};
+  p.lse = a.lse;
+  p.maps = a.maps;
+  p.dout = a.dout;
+  p.dq = a.dq;
+  p.dk = a.dk;
+  p.dv = a.dv;
+  p.dlam = a.dlam;
+  p.nq = nq;
+  p.heads = a.heads;
+  p.kv_heads = a.kv_heads;
+  p.rep = a.heads / a.kv_heads;
+  p.causal = a.causal;
+  p.scale = a.scale;
+  p.scale_log2 = a.scale * kLog2e;
+  p.err = h->derr;
+  // statistics rows: every sequence starts at a multiple of 4 (16-byte bulk copies)
+  std::vector<int32_t> st_row(a.batch);
+  std::vector<SeqRec> recs;
+  int64_t rows = 0;
+  for (int b = 0; b < a.batch; ++b) {
+    st_row[b] = static_cast<int32_t>(rows);
+    if (a.cu_q[b + 1] == a.cu_q[b]) continue;
+    recs.push_back(SeqRec{a.cu_q[b], a.cu_q[b + 1], 0, 0, a.cu_q[b], st_row[b]});
+    rows += (a.cu_q[b + 1] - a.cu_q[b] + 3) / 4 * 4;
+    if (rows > 0x7fffff00) return set_error(h, SC_EINVAL, "differential attention backward: too many rows");
+  }
+  p.np = rows + kY;  // a tile's copy may reach behind the last row
+  cudaError_t e = dev_alloc(h, reinterpret_cast<void**>(&p.st), sizeof(float) * 4 * a.heads * p.np);
   if (e != cudaSuccess) return cuda_error(h, e, "differential attention workspace");
   sc_status st = SC_OK;
   if (nq > 0) {
-    ++h->launches;
-    k_da_delta<T><<<static_cast<unsigned>((nq * a.heads + 7) / 8), 256, 0, h->stream>>>(p);
-  }
-  if (a.dlam) {
-    ++h->launches;
-    k_da_dlam<<<a.lam_count, 1024, 0, h->stream>>>(p);
-  }
-  for (int keys = 0; keys < 2 && st == SC_OK; ++keys) {
-    if (keys ? !a.dk && !a.dv : !a.dq) continue;
-    std::vector<SeqRec> recs;
     SeqPlan plan;
-    const int32_t items = row_items(a, keys != 0, &recs);
-    if (items == 0) continue;
-    st = make_plan(h, recs, &plan, &tables[keys]);
-    if (st != SC_OK) break;
-    ++h->launches;
-    const dim3 grid((items + 3) / 4, keys ? a.kv_heads : a.heads);
-    if (keys) k_da_dkv_rows<T><<<grid, 128, 0, h->stream>>>(p, plan, items);
-    else k_da_dq_rows<T><<<grid, 128, 0, h->stream>>>(p, plan, items);
+    void* table = nullptr;
+    st = make_plan(h, recs, &plan, &table);
+    if (st == SC_OK) {
+      ++h->launches;
+      k_da_stats<T><<<static_cast<unsigned>((nq * a.heads + 7) / 8), 256, 0, h->stream>>>(p, plan);
+      dev_free(h, table);
+    }
   }
+  if (st == SC_OK && a.dlam) {
+    ++h->launches;
+    k_da_dlam<<<a.lam_count, 1024, 0, h->stream>>>(p, rows);
+  }
+  if (st == SC_OK && (a.dk || a.dv)) st = launch_bwd<T, true>(h, a, p, st_row);
+  if (st == SC_OK && a.dq) st = launch_bwd<T, false>(h, a, p, st_row);
   e = cudaGetLastError();
-  dev_free(h, p.delta);
-  dev_free(h, tables[0]);
-  dev_free(h, tables[1]);
+  dev_free(h, p.st);
   if (st != SC_OK) return st;
   return e == cudaSuccess ? SC_OK : cuda_error(h, e, "differential attention backward launch");
 }
