@@ -9,14 +9,18 @@
 // One CTA per (tile of 128 rows, key / value head, range of keys).  A row is a
 // (token, head) pair: the heads that share a key / value head lie side by side
 // in a tile, so its keys and values are read once for all of them.  The two
-// maps share V, so a CTA runs both over the same key tiles, with O_1 and O_2 in
-// tensor memory (128 columns each) beside one 128-column score buffer per map:
+// maps share V, so a CTA runs both over the same key tiles (step i = tile i / 2,
+// map i % 2).  Tensor memory: O_1 and O_2 (128 columns each), one score buffer
+// of 128 columns that the maps use in turn, and 64 columns of weights per map.
+// A softmax thread takes its whole row of scores into registers at once, which
+// frees the buffer for the next step's scores long before the weights of this
+// step are done; with a score buffer per map that the weights overwrote, a map
+// waited for its P V and the scores behind it every tile (746 TFLOP/s).
 //   warp 0     TMA producer: Q_1, Q_2 once, then K_1, K_2 and V of a 128-key
 //              tile (64 KB) into a ring of three
-//   warp 1     issues the products, alternating between the maps: O_m += P_m V
-//              as soon as P_m is written (P as the A operand in tensor memory,
-//              over the scores it came from; V from shared memory, MN-major),
-//              then S_m of the next tile into the buffer that freed
+//   warp 1     issues the products: S of step i + 1 when the scores of step i
+//              are read, O_m += P_m V of step i when its weights are written (P
+//              as the A operand in tensor memory, V from shared memory, MN-major)
 //   warp 2     zeroes V rows behind the last key that any row of the tile sees
 //              (their weights are 0, but 0 * NaN would be NaN)
 //   warps 4-7, 8-11  softmax of map 1 / map 2, one row per thread: running
@@ -44,7 +48,8 @@ constexpr int kOffQ = 0;
 constexpr int kOffKV = 2 * kQBytes;
 constexpr int kOffBar = kOffKV + kStages * kStageBytes;
 constexpr int kSmem = kOffBar + 256 + 1024;
-constexpr uint32_t kTmem = 512;            // S_1 | S_2 | O_1 | O_2
+constexpr uint32_t kTmem = 512;            // S | P_1 | P_2 | O_1 | O_2
+constexpr uint32_t kColP = 128, kColO = 256;  // + 64 m, + 128 m
 constexpr float kRescale = 8.f;            // log2
 
 struct DaFwd {
@@ -91,7 +96,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t q_full = smem_u32(bars);
   const uint32_t kv_full0 = q_full + 8, kv_empty0 = kv_full0 + 8 * kStages;
   const uint32_t s_full0 = kv_empty0 + 8 * kStages, p_full0 = s_full0 + 16, o_done0 = p_full0 + 16;  // per map
-  const uint32_t done_bar = o_done0 + 16, v_req = done_bar + 8, v_fixed = v_req + 8;
+  const uint32_t s_free = o_done0 + 16, done_bar = s_free + 8, v_req = done_bar + 8, v_fixed = v_req + 8;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const SeqRec& rec = plan.at(plan.find(blockIdx.x));
   const DaTile tile(rec, blockIdx.x - rec.item0, p);
@@ -111,6 +116,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(p_full0 + 8 * m, (rows + 31) / 32);  // one arrival per warp with rows
       mbar_init(o_done0 + 8 * m, 1);
     }
+    mbar_init(s_free, (rows + 31) / 32);
     mbar_init(done_bar, 1);
     mbar_init(v_req, 1);
     mbar_init(v_fixed, 1);
@@ -125,7 +131,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_after();
   const uint32_t tmem = *s_tmem;
 
-  if (warp == 0) {
+  if (warp < 4) {
+    regs_release();
+    if (warp == 0) {
     // ----------------------------------------------------------- producer
     if (lane == 0 && nk > 0) {
       const int gk = h0 / p.rep;
@@ -149,22 +157,24 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (lane == 0 && nk > 0) {
       const bool bf16 = std::is_same_v<T, __nv_bfloat16>;
       const uint32_t id_s = idesc_f16(128, 128, bf16), id_o = idesc_f16(128, 128, bf16) | (1u << 16);  // V MN-major
-      auto issue_s = [&](int m, int j) {
+      auto issue_s = [&](int i) {
+        const int m = i & 1, j = i >> 1;
         const uint32_t kb = sbase + kOffKV + (j % kStages) * kStageBytes + m * kQBytes;
         const uint32_t qb = sbase + kOffQ + m * kQBytes;
 #pragma unroll
         for (int k = 0; k < kDaD / 16; ++k)
-          tc_mma_f16(tmem + 128u * m, smem_desc(qb + 32u * k, 1024, 2), smem_desc(kb + 32u * k, 1024, 2), id_s,
-                     k > 0 ? 1u : 0u);
+          tc_mma_f16(tmem, smem_desc(qb + 32u * k, 1024, 2), smem_desc(kb + 32u * k, 1024, 2), id_s, k > 0 ? 1u : 0u);
         tc_commit(s_full0 + 8u * m);
       };
-      auto issue_o = [&](int m, int j) {  // O_m (+)= P_m V_j
+      auto issue_o = [&](int i) {  // O_m (+)= P_m V_j
+        const int m = i & 1, j = i >> 1;
         const uint32_t vb = sbase + kOffKV + (j % kStages) * kStageBytes + 2 * kQBytes;
 #pragma unroll
         for (int k = 0; k < kTile / 16; ++k)
-          tc_mma_f16_tmem_a(tmem + 256u + 128u * m, tmem + 128u * m + 8u * k, smem_desc_mn(vb + 2048u * k, kQBytes),
-                            id_o, (j > 0 || k > 0) ? 1u : 0u);
+          tc_mma_f16_tmem_a(tmem + kColO + 128u * m, tmem + kColP + 64u * m + 8u * k,
+                            smem_desc_mn(vb + 2048u * k, kQBytes), id_o, (j > 0 || k > 0) ? 1u : 0u);
         tc_commit(o_done0 + 8u * m);
+        if (m == 1) tc_commit(kv_empty0 + 8 * (j % kStages));  // K_j and V_j are read
       };
       auto landed = [&](int j) {
         const bool r = mbar_wait(kv_full0 + 8 * (j % kStages), (j / kStages) & 1, p.err);
@@ -174,24 +184,24 @@ __global__ void __launch_bounds__(kThreads, 1)
       bool ok = mbar_wait(q_full, 0, p.err) && landed(0);
       if (ok) {
         tc_fence_after();
-        issue_s(0, 0);
-        issue_s(1, 0);
+        issue_s(0);
       }
-      for (int j = 0; ok && j < nk; ++j) {
-        if (j + 1 < nk) ok = landed(j + 1);
-        for (int m = 0; ok && m < 2; ++m) {
-          ok = mbar_wait(p_full0 + 8u * m, j & 1, p.err);
-          if (ok && m == 0 && j == nk - 1 && last_partial) ok = mbar_wait(v_fixed, 0, p.err);
+      const int steps = 2 * nk;
+      for (int i = 0; ok && i <= steps; ++i) {
+        if (i + 1 < steps) {  // scores of step i + 1, once those of step i are in registers
+          if ((i + 1) % 2 == 0) ok = landed((i + 1) / 2);
+          ok = ok && mbar_wait(s_free, i & 1, p.err);
           if (!ok) break;
           tc_fence_after();
-          issue_o(m, j);
-          if (m == 1) tc_commit(kv_empty0 + 8 * (j % kStages));  // K_j and V_j are read
-          if (j + 1 < nk) {
-            ok = mbar_wait(o_done0 + 8u * m, j & 1, p.err);  // P_m is read: its columns are free
-            if (!ok) break;
-            tc_fence_after();
-            issue_s(m, j + 1);
-          }
+          issue_s(i + 1);
+        }
+        if (i > 0) {  // weights of step i - 1
+          const int k = i - 1;
+          ok = mbar_wait(p_full0 + 8u * (k & 1), (k >> 1) & 1, p.err);
+          if (ok && k == steps - 2 && last_partial) ok = mbar_wait(v_fixed, 0, p.err);
+          if (!ok) break;
+          tc_fence_after();
+          issue_o(k);
         }
       }
       tc_commit(done_bar);  // every product ends before its tensor memory is released
@@ -214,11 +224,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (lane == 0) mbar_arrive(v_fixed);
       }
     }
-  } else if (warp >= 4) {
+    }
+  } else {
     // ------------------------------------------------------------ softmax
+    regs_take();
     const int m = (warp - 4) >> 2, row = (warp & 3) * 32 + lane;
     const uint32_t lane_base = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
-    const uint32_t sa = lane_base + 128u * m, oa = lane_base + 256u + 128u * m;
+    const uint32_t pa = lane_base + kColP + 64u * m, oa = lane_base + kColO + 128u * m;
     const bool live = row < rows;
     const int tok = tile.tok0 + row / p.pack;  // in the sequence
     const int limit = live ? min(tile.key1, key_limit(rec, tok, p.causal)) : 0;
@@ -239,41 +251,44 @@ __global__ void __launch_bounds__(kThreads, 1)
           break;
         }
         tc_fence_after();
+        float s[2][64];
+        tmem_ld64(lane_base, s[0]);
+        tmem_ld64(lane_base + 64u, s[1]);
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(s_free);
+        if (!full) {
+#pragma unroll
+          for (int i = 0; i < kTile; ++i) s[i / 64][i % 64] = i < valid ? s[i / 64][i % 64] : -INFINITY;  // 2^-inf = 0
+        }
         float mv[8];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) mv[k] = -INFINITY;
+        for (int k = 0; k < 8; ++k) mv[k] = fmaxf(s[0][2 * k], s[0][2 * k + 1]);
 #pragma unroll
-        for (int c = 0; c < kTile / 64; ++c) {
-          float s[64];
-          tmem_ld64(sa + c * 64, s);
-          if (full) {
-#pragma unroll
-            for (int i = 0; i < 64; i += 2) mv[(i >> 1) & 7] = max3(mv[(i >> 1) & 7], s[i], s[i + 1]);
-          } else {
-#pragma unroll
-            for (int i = 0; i < 64; ++i) mv[i & 7] = (c * 64 + i < valid) ? fmaxf(mv[i & 7], s[i]) : mv[i & 7];
-          }
-        }
+        for (int i = 16; i < kTile; i += 2) mv[(i >> 1) & 7] = max3(mv[(i >> 1) & 7], s[i / 64][i % 64], s[i / 64][i % 64 + 1]);
         const float top = fmaxf(fmaxf(fmaxf(mv[0], mv[1]), fmaxf(mv[2], mv[3])),
                                 fmaxf(fmaxf(mv[4], mv[5]), fmaxf(mv[6], mv[7]))) * p.scale_log2;
         const bool move = top > mx + kRescale;  // true for the first visible key (mx = -inf)
         const float m_new = move ? top : mx;
         const float alpha = move ? ex2_ftz(mx - m_new) : 1.f;
-        // S_m(j) was issued after P V of step j - 1 was done, so O_m is complete
-        if (j > 0 && __any_sync(0xffffffffu, move)) {
+        // the product of this map's last step: O_m is complete and P_m is read
+        if (j > 0) {
+          if (!wait_warp(o_done0 + 8u * m, (j - 1) & 1)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          if (__any_sync(0xffffffffu, move)) {
 #pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            float o[64];
-            tmem_ld64(oa + half * 64, o);
-            uint32_t w[32];
+            for (int q = 0; q < kDaDv / 16; ++q) {
+              float o[16];
+              uint32_t w[16];
+              tmem_ld16(oa + q * 16, o);
 #pragma unroll
-            for (int q = 0; q < 2; ++q) {
-#pragma unroll
-              for (int i = 0; i < 32; ++i) w[i] = __float_as_uint(o[q * 32 + i] * alpha);
-              tmem_st32(oa + half * 64 + q * 32, w);
+              for (int i = 0; i < 16; ++i) w[i] = __float_as_uint(o[i] * alpha);
+              tmem_st16(oa + q * 16, w);
             }
           }
-          tmem_wait_st();
         }
         unsigned long long sumv[4];
 #pragma unroll
@@ -281,23 +296,17 @@ __global__ void __launch_bounds__(kThreads, 1)
         const float base = m_new == -INFINITY ? 0.f : -m_new;  // no key seen yet: every weight is 2^-inf = 0
         const unsigned long long sc2 = f2(p.scale_log2, p.scale_log2), neg_m2 = f2(base, base);
 #pragma unroll
-        for (int c = 0; c < kTile / 64; ++c) {
-          float s[64];
-          tmem_ld64(sa + c * 64, s);
-          if (!full) {
+        for (int c = 0; c < kTile / 32; ++c) {
+          uint32_t pk[16];
 #pragma unroll
-            for (int i = 0; i < 64; ++i) s[i] = (c * 64 + i < valid) ? s[i] : -INFINITY;
-          }
-          uint32_t pk[32];
-#pragma unroll
-          for (int i = 0; i < 64; i += 2) {
+          for (int i = 0; i < 32; i += 2) {
             float x0, x1;
-            f2_split(fma_f2(f2(s[i], s[i + 1]), sc2, neg_m2), x0, x1);
+            f2_split(fma_f2(f2(s[c / 2][32 * (c % 2) + i], s[c / 2][32 * (c % 2) + i + 1]), sc2, neg_m2), x0, x1);
             const float p0 = ex2_ftz(x0), p1 = ex2_ftz(x1);
             sumv[(i >> 1) & 3] = add_f2(sumv[(i >> 1) & 3], f2(p0, p1));
             pk[i / 2] = pack2<T>(p0, p1);
           }
-          tmem_st32(sa + 32u * c, pk);  // over columns that this thread has read
+          tmem_st16(pa + 16u * c, pk);
         }
         tmem_wait_st();
         tc_fence_before();
@@ -336,8 +345,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         float o1[32], o2[32];
         __syncwarp();
         if (nk > 0) {
-          tmem_ld32(lane_base + 256u + 64u * m + 32u * c, o1);
-          tmem_ld32(lane_base + 384u + 64u * m + 32u * c, o2);
+          tmem_ld32(lane_base + kColO + 64u * m + 32u * c, o1);
+          tmem_ld32(lane_base + kColO + 128u + 64u * m + 32u * c, o2);
         }
         const int d = 64 * m + 32 * c;
         // a map without a sum has no product: its columns were never written
