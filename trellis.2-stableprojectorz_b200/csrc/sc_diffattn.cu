@@ -135,7 +135,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     regs_release();
     if (warp == 0) {
     // ----------------------------------------------------------- producer
-    if (lane == 0 && nk > 0) {
+    if (nk > 0 && elect_one()) {
       const int gk = h0 / p.rep;
       mbar_arrive_expect_tx(q_full, 2 * p.pack * p.tokens * 128);
       for (int m = 0; m < 2; ++m)
@@ -154,25 +154,25 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else if (warp == 1) {
     // ---------------------------------------------------------- MMA issuer
-    if (lane == 0 && nk > 0) {
+    if (nk > 0 && elect_one()) {
       const bool bf16 = std::is_same_v<T, __nv_bfloat16>;
       const uint32_t id_s = idesc_f16(128, 128, bf16), id_o = idesc_f16(128, 128, bf16) | (1u << 16);  // V MN-major
       auto issue_s = [&](int i) {
         const int m = i & 1, j = i >> 1;
-        const uint32_t kb = sbase + kOffKV + (j % kStages) * kStageBytes + m * kQBytes;
-        const uint32_t qb = sbase + kOffQ + m * kQBytes;
+        const uint64_t q = smem_desc(sbase + kOffQ + m * kQBytes, 1024, 2);
+        const uint64_t kd = smem_desc(sbase + kOffKV + (j % kStages) * kStageBytes + m * kQBytes, 1024, 2);
 #pragma unroll
-        for (int k = 0; k < kDaD / 16; ++k)
-          tc_mma_f16(tmem, smem_desc(qb + 32u * k, 1024, 2), smem_desc(kb + 32u * k, 1024, 2), id_s, k > 0 ? 1u : 0u);
+        for (int k = 0; k < kDaD / 16; ++k)  // 32 bytes a step, in units of 16
+          tc_mma_f16(tmem, q + 2 * k, kd + 2 * k, id_s, k > 0 ? 1u : 0u);
         tc_commit(s_full0 + 8u * m);
       };
       auto issue_o = [&](int i) {  // O_m (+)= P_m V_j
         const int m = i & 1, j = i >> 1;
-        const uint32_t vb = sbase + kOffKV + (j % kStages) * kStageBytes + 2 * kQBytes;
+        const uint64_t v = smem_desc_mn(sbase + kOffKV + (j % kStages) * kStageBytes + 2 * kQBytes, kQBytes);
 #pragma unroll
-        for (int k = 0; k < kTile / 16; ++k)
-          tc_mma_f16_tmem_a(tmem + kColO + 128u * m, tmem + kColP + 64u * m + 8u * k,
-                            smem_desc_mn(vb + 2048u * k, kQBytes), id_o, (j > 0 || k > 0) ? 1u : 0u);
+        for (int k = 0; k < kTile / 16; ++k)  // 16 keys of 128 bytes a step
+          tc_mma_f16_tmem_a(tmem + kColO + 128u * m, tmem + kColP + 64u * m + 8u * k, v + 128 * k, id_o,
+                            (j > 0 || k > 0) ? 1u : 0u);
         tc_commit(o_done0 + 8u * m);
         if (m == 1) tc_commit(kv_empty0 + 8 * (j % kStages));  // K_j and V_j are read
       };

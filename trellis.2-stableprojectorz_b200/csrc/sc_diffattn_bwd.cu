@@ -9,20 +9,24 @@
 // are kept by the forward in f32.  Every sum has one fixed order.
 //
 // Two kernels of one shape (k_da_bwd): a CTA holds 128 rows X (queries for dQ,
-// keys for dK and dV) and walks 64-row tiles of the other side Y.  Both maps
-// share dP, and dV takes one product with the combined weights, so a pair of
-// rows costs 768 flops in the dQ kernel and 1024 in the other.  Accumulating
-// dQ in the dK / dV kernel instead would save the second recomputation, but
-// needs sums across CTAs whose order changes from run to run.
-//   warp 0     TMA producer: X's Q / K pair and its dO / V once, then Y's 32 KB
-//              (and, for keys, the 64 rows' statistics) into a ring of four
-//   warp 1     issues S_m = X_m Y_m^T and dP (128 x 64 each) into tensor
-//              memory, and the accumulations dX_m += dS_m Y_m, dV += P dO with
-//              dS and P as A operands in tensor memory, Y MN-major
+// keys for dK and dV) and walks tiles of the other side Y.  Both maps share dP,
+// and dV takes one product with the combined weights, so a pair of rows costs
+// 768 flops in the dQ kernel and 1024 in the other.  Accumulating dQ in the
+// dK / dV kernel instead would save the second recomputation, but needs sums
+// across CTAs whose order changes from run to run.
+//   warp 0     TMA producer: X's Q / K pair and its dO / V once, then Y's tiles
+//              (and, for keys, the rows' statistics) into a ring
+//   warp 1     issues S_m = X_m Y_m^T and dP into tensor memory
+//   warp 3     issues the accumulations dX_m += dS_m Y_m, dV += P dO with dS and
+//              P as A operands in tensor memory, Y MN-major
 //   warp 2     zeroes Y rows behind the last visible one (0 * NaN)
-//   warps 4-11 the elementwise part, one row per lane, columns 0-31 / 32-63
-// S of the next tile is issued as soon as the weights of this one are in
-// registers, so the exponentials overlap the accumulations.
+//   warps 4-7, 8-11  the elementwise part, one row per thread: group 0 takes the
+//              even steps, group 1 the odd ones
+// Every buffer in tensor memory is single (S_1 S_2 dP P dS_1 dS_2 of 48 columns
+// beside the accumulators fill it), but a group takes its row of S, then of dP,
+// into registers at once, which frees them for the other group's step; so one
+// group's exponentials run beside the other's products.
+// Few CTAs: the walk is cut into ranges whose f32 sums k_da_bwd_join adds in order.
 // Every mbarrier wait is bounded (SC_ETIMEOUT).
 #include "sc_diffattn_dev.cuh"
 
@@ -33,18 +37,25 @@ namespace sc {
 namespace {
 
 constexpr int kX = 128;                   // rows per CTA
-constexpr int kY = 64;                    // rows per step
-constexpr int kStages = 4;
 constexpr int kThreads = 384;
 constexpr int kXBytes = kX * kDaD * 2;    // 16 KB
-constexpr int kYBytes = kY * kDaD * 2;    // 8 KB
-constexpr int kStageBytes = 4 * kYBytes + 4 * kY * 4;  // Y_1, Y_2, halves of the 128-wide one, statistics
 constexpr int kOffX = 0;                  // X_1, X_2, halves of the 128-wide one
 constexpr int kOffY = 4 * kXBytes;
-constexpr int kOffBar = kOffY + kStages * kStageBytes;
-constexpr int kSmem = kOffBar + 256 + 1024;
-// tensor memory columns
-constexpr uint32_t kTmem = 512, kColS = 0, kColDp = 128, kColP = 192, kColDs1 = 224, kColX = 256, kColV = 384;
+constexpr uint32_t kTmem = 512;
+
+template <bool KV>
+struct Cfg {
+  static constexpr int kY = 48;                        // rows of Y per step
+  static constexpr int kStages = 5;
+  static constexpr int kYBytes = kY * kDaD * 2;
+  static constexpr int kStage = 4 * kYBytes + (KV ? 1024 : 0);  // Y_1, Y_2, halves of the 128-wide one, statistics
+  static constexpr int kOffBar = kOffY + kStages * kStage;
+  static constexpr int kSmem = kOffBar + 256 + 1024;
+  // tensor memory columns: S_1 S_2 dP [P] dS_1 dS_2, then the accumulators
+  static constexpr uint32_t kS = 0, kDp = 2 * kY, kP = 3 * kY, kDs = KV ? 3 * kY + kY / 2 : 3 * kY, kAcc = 256,
+                            kV = 384;
+  static_assert(kDs + kY <= kAcc, "tensor memory");
+};
 
 struct DaBwd {
   LamRef lam;
@@ -54,6 +65,8 @@ struct DaBwd {
   float* st;           // [4][heads][np]: -lse_1, -lse_2, -delta_1, -delta_2
   int64_t np;          // rows of st: sequences start at multiples of 4
   void *dq, *dk, *dv, *dlam;
+  float* part;         // [splits][rows of X][heads of X][dX_1 dX_2 (dV)], when the walk is cut
+  int64_t nx;          // rows of X in all
   int64_t nq;
   int heads, kv_heads, rep, causal;
   float scale, scale_log2;
@@ -120,26 +133,28 @@ __global__ void __launch_bounds__(1024) k_da_dlam(const DaBwd p, int64_t rows) {
 // KV false: X = queries of one head, Y = keys; writes dQ.  KV true: X = keys of
 // one key / value head, Y = the queries of each of its heads in turn; writes
 // dK and dV.  tmX / tmXw: the 64- and 128-wide rows of X in boxes of 128; tmY /
-// tmYw likewise in boxes of 64.  Records: item0 counts tiles of X, aux = the
-// sequence's first row in st.
+// tmYw likewise in boxes of kY.  Records: item0 counts tiles of X, aux = the
+// sequence's first row in st.  blockIdx.z: range of the walk.
 template <typename T, bool KV>
 __global__ void __launch_bounds__(kThreads, 1)
     k_da_bwd(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmXw,
              const __grid_constant__ CUtensorMap tmY, const __grid_constant__ CUtensorMap tmYw, const DaBwd p,
              const __grid_constant__ SeqPlan plan) {
+  using C = Cfg<KV>;
+  constexpr int kY = C::kY, kStages = C::kStages, kYBytes = C::kYBytes;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const uint32_t sbase = smem_u32(smem);
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kOffBar);
-  uint32_t* s_tmem = reinterpret_cast<uint32_t*>(bars + 24);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::kOffBar);
+  uint32_t* s_tmem = reinterpret_cast<uint32_t*>(bars + 28);
   const uint32_t x_full = smem_u32(bars);
   const uint32_t y_full0 = x_full + 8, y_empty0 = y_full0 + 8 * kStages;
-  const uint32_t s_full = y_empty0 + 8 * kStages;  // S_1, S_2 written
-  const uint32_t s_free = s_full + 8;              // S_1, S_2 read
-  const uint32_t dp_full = s_free + 8, dp_free = dp_full + 8;  // dP written; dX_2's product (over dP's columns) done
-  const uint32_t ds_full = dp_free + 8;            // P, dS_1, dS_2 written
-  const uint32_t p_free = ds_full + 8;             // their products done
-  const uint32_t y_req = p_free + 8, y_fixed = y_req + 8, done_bar = y_fixed + 8;
+  // per group (the step's parity): S written, dP written, the step's products done
+  const uint32_t s_full0 = y_empty0 + 8 * kStages, dp_full0 = s_full0 + 16, p_free0 = dp_full0 + 16;
+  // every step in turn: S read, dP read, P and dS written
+  const uint32_t s_free = p_free0 + 16, dp_free = s_free + 8, ds_full = dp_free + 8;
+  // rows to zero: asked for (warp 1), zeroed (warp 2), seen (warp 3)
+  const uint32_t y_req = ds_full + 8, y_fixed = y_req + 8, y_ack = y_fixed + 8, done_bar = y_ack + 8;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const SeqRec& rec = plan.at(plan.find(blockIdx.x));
   const int lq = rec.q1 - rec.q0, lk = rec.k1 - rec.k0;
@@ -148,12 +163,15 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (!KV) xt = ntiles - 1 - xt;  // causal: the longest first
   const int x0 = xt * kX, nx = min(kX, (KV ? lk : lq) - x0);
   const int g = KV ? blockIdx.y : blockIdx.y / p.rep;
-  // rows [y0, y1) of Y in steps of 64, for each of nh heads
+  // rows [y0, y1) of Y in ny tiles, for each of nh heads; this CTA takes steps [t0, t0 + n)
   const int y1 = KV ? lq : key_limit(rec, x0 + nx - 1, p.causal);
   const int y0 = KV && p.causal ? max(0, x0 - lk + lq) / kY * kY : 0;
   const int ny = y1 > y0 ? (y1 - y0 + kY - 1) / kY : 0;
-  const int nh = KV ? p.rep : 1, n = ny * nh;
-  const bool last_partial = (y1 - y0) % kY != 0;
+  const int64_t all = static_cast<int64_t>(ny) * (KV ? p.rep : 1);
+  const int t0 = static_cast<int>(all * blockIdx.z / gridDim.z);
+  const int n = static_cast<int>(all * (blockIdx.z + 1) / gridDim.z) - t0;
+  const bool ragged = (y1 - y0) % kY != 0;
+  auto partial = [&](int j) { return ragged && (t0 + j) % ny == ny - 1; };  // the step's tile has rows that are not seen
 
   if (threadIdx.x == 0) {
     mbar_init(x_full, 1);
@@ -161,15 +179,18 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(y_full0 + 8 * st, 1);
       mbar_init(y_empty0 + 8 * st, 1);
     }
-    mbar_init(s_full, 1);
-    mbar_init(s_free, 8);
-    mbar_init(dp_full, 1);
-    mbar_init(dp_free, 1);
-    mbar_init(ds_full, 8);
-    mbar_init(p_free, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(s_full0 + 8 * i, 1);
+      mbar_init(dp_full0 + 8 * i, 1);
+      mbar_init(p_free0 + 8 * i, 1);
+    }
+    mbar_init(s_free, 4);
+    mbar_init(dp_free, 4);
+    mbar_init(ds_full, 4);
     mbar_init(y_req, 1);
     mbar_init(y_fixed, 1);
-    mbar_init(done_bar, 1);
+    mbar_init(y_ack, 1);
+    mbar_init(done_bar, 2);  // both issuers
     fence_mbar_init();
   }
   if (warp == 1) {
@@ -181,128 +202,153 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_after();
   const uint32_t tmem = *s_tmem;
 
-  if (warp == 0) {
-    // ----------------------------------------------------------- producer
-    if (lane == 0 && n > 0) {
-      const int xrow = (KV ? rec.k0 : rec.q0) + x0, xh = blockIdx.y;
-      mbar_arrive_expect_tx(x_full, 4 * kXBytes);
-      tma_load_3d(sbase + kOffX, &tmX, 0, 2 * xh, xrow, x_full);
-      tma_load_3d(sbase + kOffX + kXBytes, &tmX, 0, 2 * xh + 1, xrow, x_full);
-      tma_load_3d(sbase + kOffX + 2 * kXBytes, &tmXw, 0, xh, xrow, x_full);
-      tma_load_3d(sbase + kOffX + 3 * kXBytes, &tmXw, 64, xh, xrow, x_full);
-      for (int j = 0; j < n; ++j) {
-        const int st = j % kStages;
-        if (!mbar_wait(y_empty0 + 8 * st, ((j / kStages) & 1) ^ 1, p.err)) break;
-        const uint32_t yb = sbase + kOffY + st * kStageBytes, bar = y_full0 + 8 * st;
-        const int yh = KV ? g * p.rep + j / ny : g, yr = y0 + (j % ny) * kY, yrow = (KV ? rec.q0 : rec.k0) + yr;
-        mbar_arrive_expect_tx(bar, 4 * kYBytes + (KV ? 4 * kY * 4 : 0));
-        tma_load_3d(yb, &tmY, 0, 2 * yh, yrow, bar);
-        tma_load_3d(yb + kYBytes, &tmY, 0, 2 * yh + 1, yrow, bar);
-        tma_load_3d(yb + 2 * kYBytes, &tmYw, 0, yh, yrow, bar);
-        tma_load_3d(yb + 3 * kYBytes, &tmYw, 64, yh, yrow, bar);
-        if (KV)  // st rows start at multiples of 4: 16-byte aligned, and st has 64 rows behind its last
-          for (int k = 0; k < 4; ++k)
-            bulk_load(yb + 4 * kYBytes + k * kY * 4, p.st + (static_cast<int64_t>(k) * p.heads + yh) * p.np + rec.aux + yr,
-                      kY * 4, bar);
+  if (warp < 4) {
+    regs_release();
+    if (warp == 0) {
+      // --------------------------------------------------------- producer
+      if (n > 0 && elect_one()) {
+        const int xrow = (KV ? rec.k0 : rec.q0) + x0, xh = blockIdx.y;
+        mbar_arrive_expect_tx(x_full, 4 * kXBytes);
+        tma_load_3d(sbase + kOffX, &tmX, 0, 2 * xh, xrow, x_full);
+        tma_load_3d(sbase + kOffX + kXBytes, &tmX, 0, 2 * xh + 1, xrow, x_full);
+        tma_load_3d(sbase + kOffX + 2 * kXBytes, &tmXw, 0, xh, xrow, x_full);
+        tma_load_3d(sbase + kOffX + 3 * kXBytes, &tmXw, 64, xh, xrow, x_full);
+        int ty = t0 % ny, yh = KV ? g * p.rep + t0 / ny : g, st = 0, use = 0;
+        for (int j = 0; j < n; ++j) {
+          if (!mbar_wait(y_empty0 + 8 * st, (use & 1) ^ 1, p.err)) break;
+          const uint32_t yb = sbase + kOffY + st * C::kStage, bar = y_full0 + 8 * st;
+          const int yr = y0 + ty * kY, yrow = (KV ? rec.q0 : rec.k0) + yr;
+          mbar_arrive_expect_tx(bar, 4 * kYBytes + (KV ? 4 * kY * 4 : 0));
+          tma_load_3d(yb, &tmY, 0, 2 * yh, yrow, bar);
+          tma_load_3d(yb + kYBytes, &tmY, 0, 2 * yh + 1, yrow, bar);
+          tma_load_3d(yb + 2 * kYBytes, &tmYw, 0, yh, yrow, bar);
+          tma_load_3d(yb + 3 * kYBytes, &tmYw, 64, yh, yrow, bar);
+          if (KV)  // st rows start at multiples of 4: 16-byte aligned; st goes on behind its last row
+            for (int k = 0; k < 4; ++k)
+              bulk_load(yb + 4 * kYBytes + k * kY * 4,
+                        p.st + (static_cast<int64_t>(k) * p.heads + yh) * p.np + rec.aux + yr, kY * 4, bar);
+          if (++ty == ny) ty = 0, yh += KV ? 1 : 0;
+          if (++st == kStages) st = 0, ++use;
+        }
       }
-    }
-  } else if (warp == 1) {
-    // ---------------------------------------------------------- MMA issuer
-    if (lane == 0 && n > 0) {
-      const bool bf16 = std::is_same_v<T, __nv_bfloat16>;
-      const uint32_t id_s = idesc_f16(128, 64, bf16), id_x = id_s | (1u << 16),
-                     id_v = idesc_f16(128, 128, bf16) | (1u << 16);
-      auto ybase = [&](int j) { return sbase + kOffY + (j % kStages) * kStageBytes; };
-      auto issue_s = [&](int j) {
+    } else if (warp == 1) {
+      // ------------------------------------------------- S and dP of every step
+      if (n > 0 && elect_one()) {
+        const uint32_t id_s = idesc_f16(128, kY, std::is_same_v<T, __nv_bfloat16>);
+        const uint64_t x1 = smem_desc(sbase + kOffX, 1024, 2), xw = x1 + 2 * kXBytes / 16;
+        const uint64_t y1d = smem_desc(sbase + kOffY, 1024, 2);
+        int ty = t0 % ny, st = 0, use = 0, asked = 0;  // tile and ring place of the next step to land; tiles to zero
+        auto land = [&]() {
+          bool r = mbar_wait(y_full0 + 8 * st, use & 1, p.err);
+          if (r && ragged && ty == ny - 1) {
+            if (asked > 0) r = mbar_wait(y_ack, (asked - 1) & 1, p.err);
+            mbar_arrive(y_req);
+            ++asked;
+          }
+          if (++ty == ny) ty = 0;
+          if (++st == kStages) st = 0, ++use;
+          return r;
+        };
+        auto issue_s = [&](int j, uint64_t yd) {
 #pragma unroll
-        for (int m = 0; m < 2; ++m)
+          for (int m = 0; m < 2; ++m)
 #pragma unroll
-          for (int k = 0; k < kDaD / 16; ++k)
-            tc_mma_f16(tmem + kColS + 64u * m, smem_desc(sbase + kOffX + m * kXBytes + 32u * k, 1024, 2),
-                       smem_desc(ybase(j) + m * kYBytes + 32u * k, 1024, 2), id_s, k > 0 ? 1u : 0u);
-        tc_commit(s_full);
-      };
-      auto issue_dp = [&](int j) {
+            for (int k = 0; k < kDaD / 16; ++k)  // 32 bytes a step, in units of 16
+              tc_mma_f16(tmem + C::kS + kY * m, x1 + m * (kXBytes / 16) + 2 * k, yd + m * (kYBytes / 16) + 2 * k, id_s,
+                         k > 0 ? 1u : 0u);
+          tc_commit(s_full0 + 8u * (j & 1));
+        };
+        auto issue_dp = [&](int j, uint64_t yd) {
 #pragma unroll
-        for (int k = 0; k < kDaDv / 16; ++k)
-          tc_mma_f16(tmem + kColDp, smem_desc(sbase + kOffX + (2 + k / 4) * kXBytes + 32u * (k % 4), 1024, 2),
-                     smem_desc(ybase(j) + (2 + k / 4) * kYBytes + 32u * (k % 4), 1024, 2), id_s, k > 0 ? 1u : 0u);
-        tc_commit(dp_full);
-      };
-      auto landed = [&](int j) {
-        const bool r = mbar_wait(y_full0 + 8 * (j % kStages), (j / kStages) & 1, p.err);
-        if (r && last_partial && j % ny == ny - 1) mbar_arrive(y_req);
-        return r;
-      };
-      bool ok = mbar_wait(x_full, 0, p.err) && landed(0);
-      if (ok) {
-        tc_fence_after();
-        issue_s(0);
-        issue_dp(0);
-      }
-      for (int j = 0; ok && j < n; ++j) {
-        const bool more = j + 1 < n;
-        const bool partial = last_partial && j % ny == ny - 1;
-        // the zeroed rows of step j first: y_req of a later step waits for them
-        if (partial) ok = mbar_wait(y_fixed, (j / ny) & 1, p.err);
-        if (ok && more) {
-          ok = landed(j + 1) && mbar_wait(s_free, j & 1, p.err);
+          for (int k = 0; k < kDaDv / 16; ++k)
+            tc_mma_f16(tmem + C::kDp, xw + (k / 4) * (kXBytes / 16) + 2 * (k % 4),
+                       yd + (2 + k / 4) * (kYBytes / 16) + 2 * (k % 4), id_s, k > 0 ? 1u : 0u);
+          tc_commit(dp_full0 + 8u * (j & 1));
+        };
+        bool ok = mbar_wait(x_full, 0, p.err) && land();
+        if (ok) {
+          tc_fence_after();
+          issue_s(0, y1d);
+          issue_dp(0, y1d);
+        }
+        // scores and dP of step j + 1 as soon as those of step j are in registers
+        for (int j = 0; ok && j + 1 < n; ++j) {
+          const uint64_t yd = y1d + static_cast<uint32_t>(st) * (C::kStage / 16);
+          ok = land() && mbar_wait(s_free, j & 1, p.err);
           if (!ok) break;
           tc_fence_after();
-          issue_s(j + 1);
-        }
-        ok = ok && mbar_wait(ds_full, j & 1, p.err);
-        if (!ok) break;
-        tc_fence_after();
-        const uint32_t acc = j > 0 ? 1u : 0u;
-#pragma unroll
-        for (int k = 0; k < kY / 16; ++k)  // dS_2 lies over the halves of dP that its warps read
-          tc_mma_f16_tmem_a(tmem + kColX + 64u, tmem + kColDp + 32u * (k / 2) + 8u * (k % 2),
-                            smem_desc_mn(ybase(j) + kYBytes + 2048u * k, kYBytes), id_x, k > 0 ? 1u : acc);
-        tc_commit(dp_free);
-#pragma unroll
-        for (int k = 0; k < kY / 16; ++k)
-          tc_mma_f16_tmem_a(tmem + kColX, tmem + kColDs1 + 8u * k, smem_desc_mn(ybase(j) + 2048u * k, kYBytes), id_x,
-                            k > 0 ? 1u : acc);
-        if (KV) {
-#pragma unroll
-          for (int k = 0; k < kY / 16; ++k)
-            tc_mma_f16_tmem_a(tmem + kColV, tmem + kColP + 8u * k,
-                              smem_desc_mn(ybase(j) + 2 * kYBytes + 2048u * k, kYBytes), id_v, k > 0 ? 1u : acc);
-        }
-        tc_commit(p_free);
-        tc_commit(y_empty0 + 8 * (j % kStages));
-        if (more) {
+          issue_s(j + 1, yd);
           ok = mbar_wait(dp_free, j & 1, p.err);
           if (!ok) break;
           tc_fence_after();
-          issue_dp(j + 1);
+          issue_dp(j + 1, yd);
+        }
+        tc_commit(done_bar);  // every product ends before its tensor memory is released
+        mbar_wait(done_bar, 0, p.err);
+      }
+    } else if (warp == 3) {
+      // ------------------------------------------------------- the accumulations
+      if (n > 0 && elect_one()) {
+        const bool bf16 = std::is_same_v<T, __nv_bfloat16>;
+        const uint32_t id_x = idesc_f16(128, 64, bf16) | (1u << 16), id_v = idesc_f16(128, 128, bf16) | (1u << 16);
+        const uint64_t y1d = smem_desc_mn(sbase + kOffY, kYBytes);
+        int ty = t0 % ny, st = 0, fixed = 0;
+        bool ok = true;
+        for (int j = 0; ok && j < n; ++j) {
+          if (ragged && ty == ny - 1) {
+            ok = mbar_wait(y_fixed, fixed++ & 1, p.err);
+            mbar_arrive(y_ack);
+          }
+          ok = ok && mbar_wait(ds_full, j & 1, p.err);
+          if (!ok) break;
+          tc_fence_after();
+          const uint64_t yd = y1d + static_cast<uint32_t>(st) * (C::kStage / 16);
+          const uint32_t acc = j > 0 ? 1u : 0u;
+#pragma unroll
+          for (int m = 0; m < 2; ++m)
+#pragma unroll
+            for (int k = 0; k < kY / 16; ++k)  // 16 rows of 128 bytes a step
+              tc_mma_f16_tmem_a(tmem + C::kAcc + 64u * m, tmem + C::kDs + kY / 2 * m + 8u * k,
+                                yd + m * (kYBytes / 16) + 128 * k, id_x, k > 0 ? 1u : acc);
+          if (KV) {
+#pragma unroll
+            for (int k = 0; k < kY / 16; ++k)
+              tc_mma_f16_tmem_a(tmem + C::kV, tmem + C::kP + 8u * k, yd + 2 * (kYBytes / 16) + 128 * k, id_v,
+                                k > 0 ? 1u : acc);
+          }
+          tc_commit(p_free0 + 8u * (j & 1));
+          tc_commit(y_empty0 + 8 * st);
+          if (++ty == ny) ty = 0;
+          if (++st == kStages) st = 0;
+        }
+        tc_commit(done_bar);
+        mbar_wait(done_bar, 0, p.err);
+      }
+    } else if (warp == 2) {
+      // ---------------------------------------- Y rows behind the last visible one
+      if (ragged) {
+        const uint32_t valid = (y1 - y0) - (ny - 1) * kY;
+        int fixed = 0;
+        for (int j = 0; j < n; ++j) {
+          if (!partial(j)) continue;
+          int w = 1;
+          if (lane == 0) w = mbar_wait(y_req, fixed++ & 1, p.err) ? 1 : 0;
+          if (__shfl_sync(0xffffffffu, w, 0) == 0) break;
+          const uint32_t yb = sbase + kOffY + (j % kStages) * C::kStage;
+          for (uint32_t a = 128u * valid + 16u * lane; a < static_cast<uint32_t>(kYBytes); a += 512u)
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(yb + k * kYBytes + a), "r"(0u) : "memory");
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(y_fixed);
         }
       }
-      tc_commit(done_bar);  // every product ends before its tensor memory is released
-      mbar_wait(done_bar, 0, p.err);
     }
-  } else if (warp == 2) {
-    // ------------------------------------------ Y rows behind the last visible one
-    if (last_partial && n > 0) {
-      const uint32_t valid = (y1 - y0) - (ny - 1) * kY;
-      for (int hh = 0; hh < nh; ++hh) {
-        int w = 1;
-        if (lane == 0) w = mbar_wait(y_req, hh & 1, p.err) ? 1 : 0;
-        if (__shfl_sync(0xffffffffu, w, 0) == 0) break;
-        const uint32_t yb = sbase + kOffY + ((hh * ny + ny - 1) % kStages) * kStageBytes;
-        for (uint32_t a = 128u * valid + 16u * lane; a < static_cast<uint32_t>(kYBytes); a += 512u)
-#pragma unroll
-          for (int k = 0; k < 4; ++k)
-            asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(yb + k * kYBytes + a), "r"(0u) : "memory");
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(y_fixed);
-      }
-    }
-  } else if (warp >= 4) {
+  } else {
     // ------------------------------------------------- weights and score gradients
-    const int hf = (warp - 4) >> 2, row = (warp & 3) * 32 + lane, x = x0 + row;  // x: row of the sequence
+    regs_take();
+    const int grp = (warp - 4) >> 2, row = (warp & 3) * 32 + lane, x = x0 + row;  // x: row of the sequence
     const uint32_t lane_base = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
     const bool live = row < nx;
     // this row sees the Y rows [lo, hi)
@@ -324,144 +370,136 @@ __global__ void __launch_bounds__(kThreads, 1)
       return __shfl_sync(0xffffffffu, w, 0) != 0;
     };
     const unsigned long long sc2 = f2(p.scale_log2, p.scale_log2);
-    for (int j = 0; j < n; ++j) {
-      const int c0 = y0 + (j % ny) * kY + 32 * hf;  // first of this thread's 32 columns
-      const bool full = c0 >= lo_max && c0 + 32 <= hi_min;
-      const float nlam = -p.lam.get(KV ? g * p.rep + j / ny : blockIdx.y);
-      const float4* st = reinterpret_cast<const float4*>(smem + kOffY + (j % kStages) * kStageBytes + 4 * kYBytes) + 8 * hf;
-      if (!wait_warp(s_full, j & 1)) {
-        ok = false;
-        break;
-      }
+    for (int j = grp; j < n; j += 2) {
+      const int t = t0 + j, c0 = y0 + (t % ny) * kY;
+      const uint32_t turn = (j >> 1) & 1;
+      const bool full = c0 >= lo_max && c0 + kY <= hi_min;
+      const float nlam = -p.lam.get(KV ? g * p.rep + t / ny : blockIdx.y);
+      const float4* st = reinterpret_cast<const float4*>(smem + kOffY + (j % kStages) * C::kStage + 4 * kYBytes);
+      ok = wait_warp(s_full0 + 8u * grp, turn);
+      // the statistics landed with the tile: the MMA thread has seen that, this one has not
+      if (KV) ok = ok && wait_warp(y_full0 + 8 * (j % kStages), (j / kStages) & 1);
+      if (!ok) break;
       tc_fence_after();
-      // statistics of Y land with its tile: the MMA thread has seen them, this thread has not
-      if (KV && !wait_warp(y_full0 + 8 * (j % kStages), (j / kStages) & 1)) {
-        ok = false;
-        break;
-      }
-      float w[2][32];
+      float w[2][kY], dp[kY];
 #pragma unroll
-      for (int m = 0; m < 2; ++m) {
-        float s[32];
-        tmem_ld32(lane_base + kColS + 64u * m + 32u * hf, s);
-#pragma unroll
-        for (int i = 0; i < 32; i += 4) {
-          float4 l4;
-          if (KV) l4 = st[16 * m + i / 4];
-          else l4 = make_float4(nl[m], nl[m], nl[m], nl[m]);
-          float a, b, c, d;
-          f2_split(fma_f2(f2(s[i], s[i + 1]), sc2, f2(l4.x, l4.y)), a, b);
-          f2_split(fma_f2(f2(s[i + 2], s[i + 3]), sc2, f2(l4.z, l4.w)), c, d);
-          w[m][i] = ex2_ftz(a);
-          w[m][i + 1] = ex2_ftz(b);
-          w[m][i + 2] = ex2_ftz(c);
-          w[m][i + 3] = ex2_ftz(d);
-        }
-      }
+      for (int m = 0; m < 2; ++m) tmem_ld48(lane_base + C::kS + kY * m, w[m]);
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(s_free);
-      if (!full) {
+      auto weights = [&](int m) {
 #pragma unroll
-        for (int i = 0; i < 32; ++i) {
+        for (int i = 0; i < kY; i += 4) {
+          float4 l4 = make_float4(nl[m], nl[m], nl[m], nl[m]);
+          if (KV) l4 = st[kY / 4 * m + i / 4];
+          float a, b;
+          f2_split(fma_f2(f2(w[m][i], w[m][i + 1]), sc2, f2(l4.x, l4.y)), a, b);
+          w[m][i] = ex2_ftz(a);
+          w[m][i + 1] = ex2_ftz(b);
+          f2_split(fma_f2(f2(w[m][i + 2], w[m][i + 3]), sc2, f2(l4.z, l4.w)), a, b);
+          w[m][i + 2] = ex2_ftz(a);
+          w[m][i + 3] = ex2_ftz(b);
+        }
+      };
+      weights(0);
+      ok = wait_warp(dp_full0 + 8u * grp, turn);
+      if (!ok) break;
+      tc_fence_after();
+      tmem_ld48(lane_base + C::kDp, dp);
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(dp_free);
+      weights(1);
+      if (!full) {  // weight 0, and 0 * NaN of a row that is not seen
+#pragma unroll
+        for (int i = 0; i < kY; ++i) {
           const bool see = c0 + i >= lo && c0 + i < hi;
           w[0][i] = see ? w[0][i] : 0.f;
           w[1][i] = see ? w[1][i] : 0.f;
+          dp[i] = see ? dp[i] : 0.f;
         }
       }
-      if (!wait_warp(dp_full, j & 1)) {
-        ok = false;
-        break;
-      }
+      // P and dS of the step before are read
+      if (j > 0) ok = wait_warp(p_free0 + 8u * (grp ^ 1), ((j - 1) >> 1) & 1);
+      if (!ok) break;
       tc_fence_after();
-      float dp[32];
-      tmem_ld32(lane_base + kColDp + 32u * hf, dp);
-      if (!full) {  // 0 * NaN of a row that is not seen
-#pragma unroll
-        for (int i = 0; i < 32; ++i) dp[i] = (c0 + i >= lo && c0 + i < hi) ? dp[i] : 0.f;
-      }
-      uint32_t pk[16], k1[16], k2[16];
       const unsigned long long nlam2 = f2(nlam, nlam);
 #pragma unroll
-      for (int i = 0; i < 32; i += 4) {
-        float4 d1, d2;
-        if (KV) {
-          d1 = st[32 + i / 4];
-          d2 = st[48 + i / 4];
-          if (!full) {
-            float* e1 = &d1.x;
-            float* e2 = &d2.x;
+      for (int c = 0; c < kY; c += 16) {
+        uint32_t pk[8], k1[8], k2[8];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const bool see = c0 + i + k >= lo && c0 + i + k < hi;
-              e1[k] = see ? e1[k] : 0.f;
-              e2[k] = see ? e2[k] : 0.f;
+        for (int i = 0; i < 16; i += 4) {
+          float4 d1 = make_float4(nd[0], nd[0], nd[0], nd[0]), d2 = make_float4(nd[1], nd[1], nd[1], nd[1]);
+          if (KV) {
+            d1 = st[kY / 2 + (c + i) / 4];
+            d2 = st[3 * kY / 4 + (c + i) / 4];
+            if (!full) {
+              float* e1 = &d1.x;
+              float* e2 = &d2.x;
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                const bool see = c0 + c + i + k >= lo && c0 + c + i + k < hi;
+                e1[k] = see ? e1[k] : 0.f;
+                e2[k] = see ? e2[k] : 0.f;
+              }
             }
           }
-        } else {
-          d1 = make_float4(nd[0], nd[0], nd[0], nd[0]);
-          d2 = make_float4(nd[1], nd[1], nd[1], nd[1]);
-        }
 #pragma unroll
-        for (int k = 0; k < 4; k += 2) {
-          const unsigned long long dd = f2(dp[i + k], dp[i + k + 1]);
-          const unsigned long long w1 = f2(w[0][i + k], w[0][i + k + 1]);
-          const unsigned long long w2 = mul_f2(nlam2, f2(w[1][i + k], w[1][i + k + 1]));  // -lam P_2
-          float a, b;
-          f2_split(mul_f2(w1, add_f2(dd, k ? f2(d1.z, d1.w) : f2(d1.x, d1.y))), a, b);
-          k1[(i + k) / 2] = pack2<T>(a, b);
-          f2_split(mul_f2(w2, add_f2(dd, k ? f2(d2.z, d2.w) : f2(d2.x, d2.y))), a, b);
-          k2[(i + k) / 2] = pack2<T>(a, b);
-          if (KV) {
-            f2_split(add_f2(w1, w2), a, b);
-            pk[(i + k) / 2] = pack2<T>(a, b);
+          for (int k = 0; k < 4; k += 2) {
+            const int e = c + i + k;
+            const unsigned long long dd = f2(dp[e], dp[e + 1]);
+            const unsigned long long w1 = f2(w[0][e], w[0][e + 1]);
+            const unsigned long long w2 = mul_f2(nlam2, f2(w[1][e], w[1][e + 1]));  // -lam P_2
+            float a, b;
+            f2_split(mul_f2(w1, add_f2(dd, k ? f2(d1.z, d1.w) : f2(d1.x, d1.y))), a, b);
+            k1[(i + k) / 2] = pack2<T>(a, b);
+            f2_split(mul_f2(w2, add_f2(dd, k ? f2(d2.z, d2.w) : f2(d2.x, d2.y))), a, b);
+            k2[(i + k) / 2] = pack2<T>(a, b);
+            if (KV) {
+              f2_split(add_f2(w1, w2), a, b);
+              pk[(i + k) / 2] = pack2<T>(a, b);
+            }
           }
         }
+        if (KV) tmem_st8(lane_base + C::kP + c / 2, pk);
+        tmem_st8(lane_base + C::kDs + c / 2, k1);
+        tmem_st8(lane_base + C::kDs + kY / 2 + c / 2, k2);
       }
-      if (j > 0 && !wait_warp(p_free, (j - 1) & 1)) {
-        ok = false;
-        break;
-      }
-      tc_fence_after();
-      if (KV) tmem_st16(lane_base + kColP + 16u * hf, pk);
-      tmem_st16(lane_base + kColDs1 + 16u * hf, k1);
-      tmem_st16(lane_base + kColDp + 32u * hf, k2);
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(ds_full);
     }
-    ok = ok && n > 0 && wait_warp(p_free, (n - 1) & 1);
+    ok = ok && n > 0 && wait_warp(done_bar, 0);
     tc_fence_after();
-    // group hf writes dX_(hf+1), and half hf of dV's columns
-    const int64_t xr = static_cast<int64_t>(KV ? rec.k0 : rec.q0) + x;
+    // group 0 writes dX_1, group 1 dX_2, and each its half of dV's columns
     const int xheads = KV ? p.kv_heads : p.heads;
+    const int64_t at = (static_cast<int64_t>(KV ? rec.k0 : rec.q0) + x) * xheads + blockIdx.y;
     T* dx = static_cast<T*>(KV ? p.dk : p.dq);
     T* dv = static_cast<T*>(p.dv);
+    constexpr int kWide = KV ? 256 : 128;
 #pragma unroll
-    for (int part = 0; part < (KV ? 2 : 1); ++part) {
-      T* base = part ? dv : dx;
-      if (!base) continue;  // uniform over the grid
-      const float mul = part ? 1.f : p.scale;
-      T* dst = base + (part ? (xr * xheads + blockIdx.y) * kDaDv + 64 * hf
-                            : (xr * xheads + blockIdx.y) * (2 * kDaD) + kDaD * hf);
+    for (int part = 0; part < (KV ? 2 : 1); ++part)
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         float o[32];
         __syncwarp();
-        if (n > 0) tmem_ld32(lane_base + (part ? kColV : kColX) + 64u * hf + 32u * c, o);
-        if (live) {
+        if (n > 0) tmem_ld32(lane_base + (part ? C::kV : C::kAcc) + 64u * grp + 32u * c, o);
+        const int col = 64 * grp + 32 * c;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            uint32_t u[4];
+        for (int i = 0; i < 32; ++i) o[i] = ok ? o[i] * (part ? 1.f : p.scale) : 0.f;
+        if (live && p.part) {
+          float4* dst = reinterpret_cast<float4*>(p.part + (blockIdx.z * p.nx * xheads + at) * kWide + 128 * part + col);
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-              u[k] = ok ? pack2<T>(o[8 * i + 2 * k] * mul, o[8 * i + 2 * k + 1] * mul) : 0u;
-            reinterpret_cast<uint4*>(dst + 32 * c)[i] = make_uint4(u[0], u[1], u[2], u[3]);
-          }
+          for (int i = 0; i < 8; ++i) dst[i] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+        } else if (live && (part ? dv : dx)) {
+          uint4* dst = reinterpret_cast<uint4*>((part ? dv : dx) + at * 128 + col);
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            dst[i] = make_uint4(pack2<T>(o[8 * i], o[8 * i + 1]), pack2<T>(o[8 * i + 2], o[8 * i + 3]),
+                                pack2<T>(o[8 * i + 4], o[8 * i + 5]), pack2<T>(o[8 * i + 6], o[8 * i + 7]));
         }
       }
-    }
   }
   tc_fence_before();
   __syncthreads();
@@ -469,6 +507,24 @@ __global__ void __launch_bounds__(kThreads, 1)
     tc_fence_after();
     tmem_dealloc(tmem, kTmem);
   }
+}
+
+// Adds the ranges' sums in order: [splits][rows][wide] f32 -> the first 128
+// columns to dx, the others to dv (each may be null), four columns a thread.
+template <typename T>
+__global__ void __launch_bounds__(256) k_da_bwd_join(const float* part, int splits, int64_t rows, int wide, T* dx, T* dv) {
+  const int64_t i = blockIdx.x * 256ll + threadIdx.x;
+  const int64_t row = i / (wide / 4);
+  if (row >= rows) return;
+  const int col = static_cast<int>(i % (wide / 4)) * 4;
+  T* out = col < 128 ? dx : dv;
+  if (!out) return;
+  float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int k = 0; k < splits; ++k) {
+    const float4 v = *reinterpret_cast<const float4*>(part + (k * rows + row) * wide + col);
+    s = make_float4(s.x + v.x, s.y + v.y, s.z + v.z, s.w + v.w);
+  }
+  *reinterpret_cast<uint2*>(out + row * 128 + (col & 127)) = make_uint2(pack2<T>(s.x, s.y), pack2<T>(s.z, s.w));
 }
 
 bool box_map(CUtensorMap* m, bool bf16, const void* base, int width, int heads, int64_t rows, int64_t stride,
@@ -481,7 +537,8 @@ bool box_map(CUtensorMap* m, bool bf16, const void* base, int width, int heads, 
 }
 
 template <typename T, bool KV>
-sc_status launch_bwd(Handle* h, const DaArgs& a, const DaBwd& p, const std::vector<int32_t>& st_row) {
+sc_status launch_bwd(Handle* h, const DaArgs& a, DaBwd p, const std::vector<int32_t>& st_row) {
+  constexpr int kY = Cfg<KV>::kY;
   const bool bf16 = std::is_same_v<T, __nv_bfloat16>;
   const int64_t nq = a.cu_q[a.batch], nkv = a.cu_kv[a.batch];
   std::vector<SeqRec> recs;
@@ -493,11 +550,19 @@ sc_status launch_bwd(Handle* h, const DaArgs& a, const DaBwd& p, const std::vect
   std::stable_sort(recs.begin(), recs.end(), [](const SeqRec& x, const SeqRec& y) {
     return KV ? x.q1 - x.q0 > y.q1 - y.q0 : x.k1 - x.k0 > y.k1 - y.k0;
   });
-  int64_t items = 0;
+  int64_t items = 0, steps = 0;
+  const int xheads = KV ? a.kv_heads : a.heads;
   for (SeqRec& r : recs) {
+    const int64_t tiles = ((KV ? r.k1 - r.k0 : r.q1 - r.q0) + kX - 1) / kX;
     r.item0 = static_cast<int32_t>(items);
-    items += ((KV ? r.k1 - r.k0 : r.q1 - r.q0) + kX - 1) / kX;
+    items += tiles;
+    steps += tiles * (((KV ? r.q1 - r.q0 : r.k1 - r.k0) + kY - 1) / kY) * (KV ? p.rep : 1);
   }
+  // Fewer CTAs than SMs: the walks are cut so that two CTAs a SM have work, in
+  // ranges of eight steps at least (their sums cost a write and a read).
+  int64_t splits = 1;
+  if (items * xheads < h->num_sms)
+    splits = std::max<int64_t>(1, std::min<int64_t>({2ll * h->num_sms / (items * xheads), steps / items / 8, 32}));
   // a side without rows is never read, but its maps want an address
   const void* some = nq > 0 ? a.q : a.k;
   const void *q = nq > 0 ? a.q : some, *go = nq > 0 ? a.dout : some, *k = nkv > 0 ? a.k : some,
@@ -515,14 +580,32 @@ sc_status launch_bwd(Handle* h, const DaArgs& a, const DaBwd& p, const std::vect
   void* table = nullptr;
   const sc_status st = make_plan(h, recs, &plan, &table);
   if (st != SC_OK) return st;
-  cudaError_t e = cudaFuncSetAttribute(k_da_bwd<T, KV>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+  cudaError_t e = cudaSuccess;
+  p.nx = KV ? nkv : nq;
+  const int wide = KV ? 256 : 128;
+  if (splits > 1) {
+    e = dev_alloc(h, reinterpret_cast<void**>(&p.part), sizeof(float) * splits * p.nx * xheads * wide);
+    if (e != cudaSuccess) {
+      dev_free(h, table);
+      return cuda_error(h, e, "differential attention workspace");
+    }
+  }
+  e = cudaFuncSetAttribute(k_da_bwd<T, KV>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<KV>::kSmem);
   if (e == cudaSuccess) {
     ++h->launches;
-    const dim3 grid(static_cast<unsigned>(items), KV ? a.kv_heads : a.heads);
-    if (KV) k_da_bwd<T, KV><<<grid, kThreads, kSmem, h->stream>>>(mk, mv, mq, mo, p, plan);
-    else k_da_bwd<T, KV><<<grid, kThreads, kSmem, h->stream>>>(mq, mo, mk, mv, p, plan);
+    const dim3 grid(static_cast<unsigned>(items), xheads, static_cast<unsigned>(splits));
+    if (KV) k_da_bwd<T, KV><<<grid, kThreads, Cfg<KV>::kSmem, h->stream>>>(mk, mv, mq, mo, p, plan);
+    else k_da_bwd<T, KV><<<grid, kThreads, Cfg<KV>::kSmem, h->stream>>>(mq, mo, mk, mv, p, plan);
+    if (splits > 1) {
+      ++h->launches;
+      const int64_t rows = p.nx * xheads;
+      k_da_bwd_join<T><<<static_cast<unsigned>((rows * (wide / 4) + 255) / 256), 256, 0, h->stream>>>(
+          p.part, static_cast<int>(splits), rows, wide, static_cast<T*>(KV ? p.dk : p.dq),
+          static_cast<T*>(KV ? p.dv : nullptr));
+    }
     e = cudaGetLastError();
   }
+  dev_free(h, p.part);
   dev_free(h, table);
   return e == cudaSuccess ? SC_OK : cuda_error(h, e, "differential attention backward launch");
 }
@@ -558,7 +641,7 @@ sc_status run_backward(Handle* h, const DaArgs& a) {
     rows += (a.cu_q[b + 1] - a.cu_q[b] + 3) / 4 * 4;
     if (rows > 0x7fffff00) return set_error(h, SC_EINVAL, "differential attention backward: too many rows");
   }
-  p.np = rows + kY;  // a tile's copy may reach behind the last row
+  p.np = rows + Cfg<true>::kY;  // a tile's copy may reach behind the last row
   cudaError_t e = dev_alloc(h, reinterpret_cast<void**>(&p.st), sizeof(float) * 4 * a.heads * p.np);
   if (e != cudaSuccess) return cuda_error(h, e, "differential attention workspace");
   sc_status st = SC_OK;
