@@ -370,15 +370,27 @@ __global__ void __launch_bounds__(kThreads, 1)
       return __shfl_sync(0xffffffffu, w, 0) != 0;
     };
     const unsigned long long sc2 = f2(p.scale_log2, p.scale_log2);
+    // tile and head of the group's step, its place in the ring
+    int ty = n > 0 ? (t0 + grp) % ny : 0, head = KV ? g * p.rep + (n > 0 ? (t0 + grp) / ny : 0) : blockIdx.y;
+    int place = grp, use = 0;
+    float nlam = n > grp ? -p.lam.get(head) : 0.f;
     for (int j = grp; j < n; j += 2) {
-      const int t = t0 + j, c0 = y0 + (t % ny) * kY;
+      if (j > grp) {
+        ty += 2;
+        place += 2;
+        if (place >= kStages) place -= kStages, use ^= 1;
+        while (ty >= ny) {
+          ty -= ny;
+          if (KV) nlam = -p.lam.get(++head);
+        }
+      }
+      const int c0 = y0 + ty * kY;
       const uint32_t turn = (j >> 1) & 1;
       const bool full = c0 >= lo_max && c0 + kY <= hi_min;
-      const float nlam = -p.lam.get(KV ? g * p.rep + t / ny : blockIdx.y);
-      const float4* st = reinterpret_cast<const float4*>(smem + kOffY + (j % kStages) * C::kStage + 4 * kYBytes);
+      const float4* st = reinterpret_cast<const float4*>(smem + kOffY + place * C::kStage + 4 * kYBytes);
       ok = wait_warp(s_full0 + 8u * grp, turn);
       // the statistics landed with the tile: the MMA thread has seen that, this one has not
-      if (KV) ok = ok && wait_warp(y_full0 + 8 * (j % kStages), (j / kStages) & 1);
+      if (KV) ok = ok && wait_warp(y_full0 + 8 * place, use);
       if (!ok) break;
       tc_fence_after();
       float w[2][kY], dp[kY];
@@ -419,14 +431,10 @@ __global__ void __launch_bounds__(kThreads, 1)
           dp[i] = see ? dp[i] : 0.f;
         }
       }
-      // P and dS of the step before are read
-      if (j > 0) ok = wait_warp(p_free0 + 8u * (grp ^ 1), ((j - 1) >> 1) & 1);
-      if (!ok) break;
-      tc_fence_after();
       const unsigned long long nlam2 = f2(nlam, nlam);
+      uint32_t pk[kY / 16][8], k1[kY / 16][8], k2[kY / 16][8];
 #pragma unroll
       for (int c = 0; c < kY; c += 16) {
-        uint32_t pk[8], k1[8], k2[8];
 #pragma unroll
         for (int i = 0; i < 16; i += 4) {
           float4 d1 = make_float4(nd[0], nd[0], nd[0], nd[0]), d2 = make_float4(nd[1], nd[1], nd[1], nd[1]);
@@ -452,18 +460,26 @@ __global__ void __launch_bounds__(kThreads, 1)
             const unsigned long long w2 = mul_f2(nlam2, f2(w[1][e], w[1][e + 1]));  // -lam P_2
             float a, b;
             f2_split(mul_f2(w1, add_f2(dd, k ? f2(d1.z, d1.w) : f2(d1.x, d1.y))), a, b);
-            k1[(i + k) / 2] = pack2<T>(a, b);
+            k1[c / 16][(i + k) / 2] = pack2<T>(a, b);
             f2_split(mul_f2(w2, add_f2(dd, k ? f2(d2.z, d2.w) : f2(d2.x, d2.y))), a, b);
-            k2[(i + k) / 2] = pack2<T>(a, b);
+            k2[c / 16][(i + k) / 2] = pack2<T>(a, b);
             if (KV) {
               f2_split(add_f2(w1, w2), a, b);
-              pk[(i + k) / 2] = pack2<T>(a, b);
+              pk[c / 16][(i + k) / 2] = pack2<T>(a, b);
             }
           }
         }
-        if (KV) tmem_st8(lane_base + C::kP + c / 2, pk);
-        tmem_st8(lane_base + C::kDs + c / 2, k1);
-        tmem_st8(lane_base + C::kDs + kY / 2 + c / 2, k2);
+      }
+      // the columns of the step before are read: only these stores and the
+      // products stand between one step's wait here and the next one's
+      if (j > 0) ok = wait_warp(p_free0 + 8u * (grp ^ 1), ((j - 1) >> 1) & 1);
+      if (!ok) break;
+      tc_fence_after();
+#pragma unroll
+      for (int c = 0; c < kY / 16; ++c) {
+        if (KV) tmem_st8(lane_base + C::kP + 8 * c, pk[c]);
+        tmem_st8(lane_base + C::kDs + 8 * c, k1[c]);
+        tmem_st8(lane_base + C::kDs + kY / 2 + 8 * c, k2[c]);
       }
       tmem_wait_st();
       tc_fence_before();
