@@ -9,13 +9,23 @@
 //   dw = sum_seq B, db = sum_seq A,
 //   dx = rstd (w dz - (sum_c w A) / n - xhat (sum_c w B) / n).
 //
-// Rows are cut into chunks, one CTA each.  The first kernel reduces a chunk
-// to one (mean, M2) per group (backward: the sums); the second combines its
-// sequence's chunks in a fixed order and writes its rows, last chunks first,
-// so that it finds the most recently read rows in L2.  Every statistic is
-// f32: per thread and channel a running mean and M2 (no difference of large
-// sums), merged by counts.  The order of every sum is fixed by the sizes, so
-// results repeat bit for bit.
+// Bound: HBM (x read and y written; backward x and dy read, dx written), as long
+// as the second pass over x finds part of it in L2.
+//
+// Rows are cut into chunks, one CTA each, two CTAs per SM.  The first kernel
+// reduces a chunk to one (mean, M2) per group (backward: the sums); the second
+// combines its sequence's chunks in a fixed order and writes its rows, last
+// chunks first, so that it finds the most recently read rows in L2; it is
+// launched early (programmatic dependent launch) and waits for the first.
+// Short sequences take one kernel: a cluster of up to eight CTAs per sequence
+// that exchanges the chunks' (mean, M2) through distributed shared memory.
+// Every statistic is f32: per thread and channel a running mean and M2 (no
+// difference of large sums), merged by counts.  The order of every sum is fixed
+// by the sizes, so results repeat bit for bit.  The arithmetic runs on packed
+// f32 pairs, and a vector whose channels share groups keeps their statistics
+// once: 64 registers, so that two CTAs of 512 threads fit an SM.
+#include <cooperative_groups.h>
+#include "sc_attn_dev.cuh"
 #include "sc_common.cuh"
 #include "sc_internal.h"
 #include "sc_plan.cuh"
@@ -85,8 +95,66 @@ __device__ __forceinline__ float warp_sum(float v) {
   return v;
 }
 
-// 1 / (1 + e^-z); e^-z overflowing gives 0
-__device__ __forceinline__ float sigmoid_f(float z) { return __fdividef(1.f, 1.f + __expf(-z)); }
+using F2 = unsigned long long;  // two f32
+
+__device__ __forceinline__ F2 mul_f2(F2 a, F2 b) {
+  F2 d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ F2 neg_f2(F2 a) { return a ^ 0x8000000080000000ull; }
+
+// 1 / (1 + e^-z) of a pair; e^-z overflowing gives 0
+__device__ __forceinline__ F2 sigmoid_f2(F2 z) {
+  float a, b;
+  f2_split(mul_f2(z, f2(-1.4426950408889634f, -1.4426950408889634f)), a, b);
+  f2_split(add_f2(f2(ex2_ftz(a), ex2_ftz(b)), f2(1.f, 1.f)), a, b);
+  float ra, rb;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(ra) : "f"(a));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(rb) : "f"(b));
+  return f2(ra, rb);
+}
+
+// Pair i of a vector (the last of an odd vector twice) / a pair back into it.
+template <typename T, int V>
+__device__ __forceinline__ F2 get_pair(const Pack<T, V>& v, int i) {
+  if constexpr (sizeof(T) == 4) {
+    return f2(v.t[2 * i], v.t[V > 1 ? 2 * i + 1 : 0]);
+  } else if constexpr (std::is_same_v<T, __nv_bfloat16> && V > 1) {
+    const uint32_t w = reinterpret_cast<const uint32_t*>(&v.w)[i];
+    return f2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+  } else {
+    return f2(Cvt<T>::to_f(v.t[2 * i]), Cvt<T>::to_f(v.t[V > 1 ? 2 * i + 1 : 0]));
+  }
+}
+template <typename T, int V>
+__device__ __forceinline__ void put_pair(Pack<T, V>& v, int i, F2 x) {
+  float a, b;
+  f2_split(x, a, b);
+  if constexpr (sizeof(T) == 2 && V > 1) {
+    reinterpret_cast<uint32_t*>(&v.w)[i] = pack2<T>(a, b);
+  } else {
+    v.t[2 * i] = Cvt<T>::from_f(a);
+    if constexpr (V > 1) v.t[2 * i + 1] = Cvt<T>::from_f(b);
+  }
+}
+
+// Statistics of the groups that a vector of V channels meets: GS consecutive
+// channels share a group (GS even), or each channel has its own (GS = 1).
+template <int V, int GS>
+struct Span {
+  static constexpr int NP = (V + 1) / 2;                 // pairs of the vector
+  static constexpr int NR = GS > 1 ? V / GS : NP;        // pairs of statistics
+  static __device__ __forceinline__ int of(int i) { return GS > 1 ? 2 * i / GS : i; }
+  // s[group] of the vector's channels, times f
+  static __device__ __forceinline__ void load(const float* s, int stride, int c0, int cg, F2 (&out)[NR]) {
+#pragma unroll
+    for (int r = 0; r < NR; ++r) {
+      const float a = s[(c0 + (GS > 1 ? r * GS : 2 * r)) / cg * stride];
+      out[r] = f2(a, GS > 1 || V == 1 ? a : s[(c0 + 2 * r + 1) / cg * stride]);
+    }
+  }
+};
 
 // The thread's place: column vector tx of TX (then tx + TX, ...; only when a
 // row has more vectors than the block threads), row lane ty of TY.
@@ -103,6 +171,11 @@ struct Place {
 };
 
 struct Chunk {
+  // rank's share of one sequence
+  __device__ __forceinline__ Chunk(const SeqRec& r, int rank, int chunk)
+      : row0(r.q0 + static_cast<int64_t>(rank) * chunk),
+        rows(static_cast<int>(max(int64_t(0), min(static_cast<int64_t>(chunk), r.q1 - row0)))),
+        seq(r.aux), first_item(0), seq_items(0), seq_rows(r.q1 - r.q0) {}
   int64_t row0;
   int rows, seq, first_item, seq_items;
   int64_t seq_rows;
@@ -117,51 +190,65 @@ struct Chunk {
   }
 };
 
+__device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void grid_release() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+// Calls f(column vector, first row pointer offsets) ... rows of the chunk in
+// batches of U loads: load(u, row) for each of a batch, then use(u, row).
+template <int U, typename L, typename F>
+__device__ __forceinline__ void for_rows(int rows, const Place& at, L&& load, F&& use) {
+  int r = at.ty;
+  for (; r + (U - 1) * at.TY < rows; r += U * at.TY) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) load(u, r + u * at.TY);
+#pragma unroll
+    for (int u = 0; u < U; ++u) use(u, r + u * at.TY);
+  }
+  for (; r < rows; r += at.TY) {
+    load(0, r);
+    use(0, r);
+  }
+}
+
+// (mean, M2) of every group of the chunk, to dst[g * stride].  sm: [TY][C]
+// means, then [TY][C] M2.
 template <typename T, int V>
-__global__ void __launch_bounds__(kGnThreads)
-    k_gn_stats(const GnParams p, const __grid_constant__ SeqPlan plan) {
-  extern __shared__ float sm[];  // [TY][C] means, then [TY][C] M2
+__device__ __forceinline__ void gn_chunk_stats(const GnParams& p, const Chunk& ch, float* sm, float2* dst,
+                                               int64_t stride) {
+  constexpr int NP = (V + 1) / 2;
   const int nvec = p.c / V;
   const Place at(nvec);
-  const Chunk ch(plan, blockIdx.x, p.chunk);
   float* s_mean = sm;
   float* s_m2 = sm + at.TY * p.c;
   const T* x = static_cast<const T*>(p.x);
   if (at.live) {
     for (int cv = at.tx; cv < nvec; cv += at.TX) {
-      float mean[V], m2[V];
+      F2 mean[NP], m2[NP];
 #pragma unroll
-      for (int e = 0; e < V; ++e) mean[e] = m2[e] = 0.f;
+      for (int i = 0; i < NP; ++i) mean[i] = m2[i] = 0ull;
       const T* px = x + ch.row0 * p.xs + cv * V;
       float n = 0.f;
-      auto add = [&](const Pack<T, V>& v) {
-        n += 1.f;
-        const float inv = __fdividef(1.f, n);
+      Pack<T, V> v[4];
+      for_rows<4>(
+          ch.rows, at, [&](int u, int r) { v[u].load(px + static_cast<int64_t>(r) * p.xs); },
+          [&](int u, int) {
+            n += 1.f;
+            const float inv = __fdividef(1.f, n);
+            const F2 inv2 = f2(inv, inv);
 #pragma unroll
-        for (int e = 0; e < V; ++e) {
-          const float f = Cvt<T>::to_f(v.t[e]), d = f - mean[e];
-          mean[e] = fmaf(d, inv, mean[e]);
-          m2[e] = fmaf(d, f - mean[e], m2[e]);
-        }
-      };
-      constexpr int U = 4;
-      int r = at.ty;
-      for (; r + (U - 1) * at.TY < ch.rows; r += U * at.TY) {
-        Pack<T, V> v[U];
-#pragma unroll
-        for (int u = 0; u < U; ++u) v[u].load(px + static_cast<int64_t>(r + u * at.TY) * p.xs);
-#pragma unroll
-        for (int u = 0; u < U; ++u) add(v[u]);
-      }
-      for (; r < ch.rows; r += at.TY) {
-        Pack<T, V> v;
-        v.load(px + static_cast<int64_t>(r) * p.xs);
-        add(v);
-      }
+            for (int i = 0; i < NP; ++i) {
+              const F2 f = get_pair<T, V>(v[u], i), d = add_f2(f, neg_f2(mean[i]));
+              mean[i] = fma_f2(d, inv2, mean[i]);
+              m2[i] = fma_f2(d, add_f2(f, neg_f2(mean[i])), m2[i]);
+            }
+          });
 #pragma unroll
       for (int e = 0; e < V; ++e) {
-        s_mean[at.ty * p.c + cv * V + e] = mean[e];
-        s_m2[at.ty * p.c + cv * V + e] = m2[e];
+        float a, b;
+        f2_split(mean[e / 2], a, b);
+        s_mean[at.ty * p.c + cv * V + e] = e & 1 ? b : a;
+        f2_split(m2[e / 2], a, b);
+        s_m2[at.ty * p.c + cv * V + e] = e & 1 ? b : a;
       }
     }
   }
@@ -182,29 +269,76 @@ __global__ void __launch_bounds__(kGnThreads)
       q += fmaf(static_cast<float>((ch.rows - ty + at.TY - 1) / at.TY) * d, d, s_m2[ty * p.c + c]);
     }
     q = warp_sum(q);
-    if (lane == 0) p.part[static_cast<int64_t>(g) * p.items + blockIdx.x] = make_float2(mean, q);
+    if (lane == 0) dst[g * stride] = make_float2(mean, q);
   }
 }
 
-// Mean and rstd of the chunk's sequence from its chunks' (mean, M2), into
-// s_mean / s_rstd [G]; every CTA of a sequence computes the same values.
-__device__ __forceinline__ void gn_combine(const GnParams& p, const Chunk& ch, float* s_mean, float* s_rstd) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const float n = static_cast<float>(ch.seq_rows) * p.cg;
-  for (int g = warp; g < p.groups; g += kGnWarps) {
-    const float2* part = p.part + static_cast<int64_t>(g) * p.items + ch.first_item;
-    float s = 0.f;
-    for (int i = lane; i < ch.seq_items; i += 32) {
-      const float ni = static_cast<float>(min(static_cast<int64_t>(p.chunk),
-                                              ch.seq_rows - static_cast<int64_t>(i) * p.chunk)) * p.cg;
-      s = fmaf(ni, part[i].x, s);
+// y of the chunk's rows from s_mean / s_rstd [G].
+template <typename T, int V, int GS>
+__device__ __forceinline__ void gn_chunk_apply(const GnParams& p, const Chunk& ch, const float* s_mean,
+                                               const float* s_rstd) {
+  using S = Span<V, GS>;
+  const int nvec = p.c / V;
+  const Place at(nvec);
+  if (!at.live) return;
+  const T* x = static_cast<const T*>(p.x);
+  T* y = static_cast<T*>(p.y);
+  for (int cv = at.tx; cv < nvec; cv += at.TX) {
+    F2 mean[S::NR], a[S::NP], b[S::NP];
+    S::load(s_mean, 1, cv * V, p.cg, mean);
+    {
+      F2 rstd[S::NR];
+      S::load(s_rstd, 1, cv * V, p.cg, rstd);
+#pragma unroll
+      for (int i = 0; i < S::NP; ++i) {
+        const int c = cv * V + 2 * i, d = V > 1 ? c + 1 : c;
+        a[i] = mul_f2(rstd[S::of(i)], f2(load_w(p.w, p.wdtype, c, 1.f), load_w(p.w, p.wdtype, d, 1.f)));
+        b[i] = f2(load_w(p.b, p.wdtype, c, 0.f), load_w(p.b, p.wdtype, d, 0.f));
+      }
     }
+    const T* px = x + ch.row0 * p.xs + cv * V;
+    T* py = y + ch.row0 * p.c + cv * V;
+    Pack<T, V> v[4];
+    for_rows<4>(
+        ch.rows, at, [&](int u, int r) { v[u].load(px + static_cast<int64_t>(r) * p.xs); },
+        [&](int u, int r) {
+          Pack<T, V> o;
+#pragma unroll
+          for (int i = 0; i < S::NP; ++i) {
+            F2 z = fma_f2(add_f2(get_pair<T, V>(v[u], i), neg_f2(mean[S::of(i)])), a[i], b[i]);
+            if (p.silu) z = mul_f2(z, sigmoid_f2(z));
+            put_pair<T, V>(o, i, z);
+          }
+          o.store(py + static_cast<int64_t>(r) * p.c);
+        });
+  }
+}
+
+template <typename T, int V>
+__global__ void __launch_bounds__(kGnThreads, 2)
+    k_gn_stats(const GnParams p, const __grid_constant__ SeqPlan plan) {
+  extern __shared__ float sm[];
+  grid_release();
+  const Chunk ch(plan, blockIdx.x, p.chunk);
+  gn_chunk_stats<T, V>(p, ch, sm, p.part + blockIdx.x, p.items);
+}
+
+// Mean and rstd of every group of a sequence from its chunks' (mean, M2):
+// part(i, g) for chunk i of `chunks`, chunk_rows rows each but the last.
+template <typename P>
+__device__ __forceinline__ void gn_combine(const GnParams& p, int64_t rows, int chunks, int64_t chunk_rows, P&& part,
+                                           float* s_mean, float* s_rstd) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const float n = static_cast<float>(rows) * p.cg;
+  for (int g = warp; g < p.groups; g += kGnWarps) {
+    float s = 0.f;
+    for (int i = lane; i < chunks; i += 32)
+      s = fmaf(static_cast<float>(max(int64_t(0), min(chunk_rows, rows - i * chunk_rows))) * p.cg, part(i, g).x, s);
     const float mean = warp_sum(s) / n;
     float q = 0.f;
-    for (int i = lane; i < ch.seq_items; i += 32) {
-      const float ni = static_cast<float>(min(static_cast<int64_t>(p.chunk),
-                                              ch.seq_rows - static_cast<int64_t>(i) * p.chunk)) * p.cg;
-      const float2 v = part[i];
+    for (int i = lane; i < chunks; i += 32) {
+      const float ni = static_cast<float>(max(int64_t(0), min(chunk_rows, rows - i * chunk_rows))) * p.cg;
+      const float2 v = part(i, g);
       q += fmaf(ni * (v.x - mean), v.x - mean, v.y);
     }
     const float rstd = rsqrtf(warp_sum(q) / n + p.eps);
@@ -213,79 +347,71 @@ __device__ __forceinline__ void gn_combine(const GnParams& p, const Chunk& ch, f
       s_rstd[g] = rstd;
     }
   }
-  __syncthreads();
 }
 
-template <typename T, int V>
-__global__ void __launch_bounds__(kGnThreads)
+__device__ __forceinline__ void gn_keep_stats(const GnParams& p, int seq, const float* s_mean, const float* s_rstd) {
+  for (int g = threadIdx.x; g < p.groups; g += kGnThreads) {
+    float* st = p.stats + (static_cast<int64_t>(seq) * p.groups + g) * 2;
+    st[0] = s_mean[g];
+    st[1] = s_rstd[g];
+  }
+}
+
+template <typename T, int V, int GS>
+__global__ void __launch_bounds__(kGnThreads, 2)
     k_gn_apply(const GnParams p, const __grid_constant__ SeqPlan plan) {
   extern __shared__ float sm[];
   float* s_mean = sm;
   float* s_rstd = sm + p.groups;
   const int item = p.items - 1 - blockIdx.x;
   const Chunk ch(plan, item, p.chunk);
-  gn_combine(p, ch, s_mean, s_rstd);
-  if (p.stats && item == ch.first_item)
-    for (int g = threadIdx.x; g < p.groups; g += kGnThreads) {
-      float* st = p.stats + (static_cast<int64_t>(ch.seq) * p.groups + g) * 2;
-      st[0] = s_mean[g];
-      st[1] = s_rstd[g];
-    }
-  const int nvec = p.c / V;
-  const Place at(nvec);
-  if (!at.live) return;
-  const T* x = static_cast<const T*>(p.x);
-  T* y = static_cast<T*>(p.y);
-  for (int cv = at.tx; cv < nvec; cv += at.TX) {
-    float mean[V], a[V], b[V];
-#pragma unroll
-    for (int e = 0; e < V; ++e) {
-      const int c = cv * V + e, g = c / p.cg;
-      mean[e] = s_mean[g];
-      a[e] = s_rstd[g] * load_w(p.w, p.wdtype, c, 1.f);
-      b[e] = load_w(p.b, p.wdtype, c, 0.f);
-    }
-    const T* px = x + ch.row0 * p.xs + cv * V;
-    T* py = y + ch.row0 * p.c + cv * V;
-    auto put = [&](Pack<T, V>& v, int r) {
-#pragma unroll
-      for (int e = 0; e < V; ++e) {
-        float z = fmaf(Cvt<T>::to_f(v.t[e]) - mean[e], a[e], b[e]);
-        if (p.silu) z *= sigmoid_f(z);
-        v.t[e] = Cvt<T>::from_f(z);
-      }
-      v.store(py + static_cast<int64_t>(r) * p.c);
-    };
-    constexpr int U = 4;
-    int r = at.ty;
-    for (; r + (U - 1) * at.TY < ch.rows; r += U * at.TY) {
-      Pack<T, V> v[U];
-#pragma unroll
-      for (int u = 0; u < U; ++u) v[u].load(px + static_cast<int64_t>(r + u * at.TY) * p.xs);
-#pragma unroll
-      for (int u = 0; u < U; ++u) put(v[u], r + u * at.TY);
-    }
-    for (; r < ch.rows; r += at.TY) {
-      Pack<T, V> v;
-      v.load(px + static_cast<int64_t>(r) * p.xs);
-      put(v, r);
-    }
-  }
+  grid_wait();
+  gn_combine(p, ch.seq_rows, ch.seq_items, p.chunk,
+             [&](int i, int g) { return p.part[static_cast<int64_t>(g) * p.items + ch.first_item + i]; }, s_mean, s_rstd);
+  __syncthreads();
+  if (p.stats && item == ch.first_item) gn_keep_stats(p, ch.seq, s_mean, s_rstd);
+  gn_chunk_apply<T, V, GS>(p, ch, s_mean, s_rstd);
 }
 
-// dz of one value: x -> xhat, and the gradient through the activation.
-__device__ __forceinline__ float gn_dz(float x, float dy, float mean, float rstd, float w, float b, int silu,
-                                       float& xhat) {
-  xhat = (x - mean) * rstd;
+// One cluster per sequence (records: one item each); rank r takes the rows
+// [r chunk, (r + 1) chunk) of it.
+template <typename T, int V, int GS>
+__global__ void __launch_bounds__(kGnThreads, 2)
+    k_gn_cluster(const GnParams p, const __grid_constant__ SeqPlan plan, int ranks) {
+  extern __shared__ float sm[];
+  namespace cg = cooperative_groups;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int rank = static_cast<int>(cluster.block_rank());
+  const SeqRec& rec = plan.at(blockIdx.x / ranks);
+  const int64_t rows = rec.q1 - rec.q0, chunk_rows = (rows + ranks - 1) / ranks;
+  Chunk ch(rec, rank, static_cast<int>(chunk_rows));
+  float2* s_part = reinterpret_cast<float2*>(sm);
+  float* s_mean = sm + 2 * p.groups;
+  float* s_rstd = s_mean + p.groups;
+  if (ch.rows > 0) gn_chunk_stats<T, V>(p, ch, s_rstd + p.groups, s_part, 1);
+  else for (int g = threadIdx.x; g < p.groups; g += kGnThreads) s_part[g] = make_float2(0.f, 0.f);
+  cluster.sync();
+  gn_combine(p, rows, ranks, chunk_rows, [&](int i, int g) { return cluster.map_shared_rank(s_part, i)[g]; }, s_mean,
+             s_rstd);
+  cluster.sync();  // every rank has read the others' before any leaves
+  if (p.stats && rank == 0) gn_keep_stats(p, rec.aux, s_mean, s_rstd);
+  if (ch.rows > 0) gn_chunk_apply<T, V, GS>(p, ch, s_mean, s_rstd);
+}
+
+// dz of a pair: x -> xhat, and the gradient through the activation.
+__device__ __forceinline__ F2 gn_dz(F2 x, F2 dy, F2 mean, F2 rstd, F2 w, F2 b, int silu, F2& xhat) {
+  xhat = mul_f2(add_f2(x, neg_f2(mean)), rstd);
   if (!silu) return dy;
-  const float z = fmaf(xhat, w, b), s = sigmoid_f(z);
-  return dy * s * fmaf(z, 1.f - s, 1.f);
+  const F2 one = f2(1.f, 1.f), z = fma_f2(xhat, w, b), s = sigmoid_f2(z);
+  return mul_f2(mul_f2(dy, s), fma_f2(z, add_f2(one, neg_f2(s)), one));
 }
 
-template <typename T, int V>
-__global__ void __launch_bounds__(kGnThreads)
+template <typename T, int V, int GS>
+__global__ void __launch_bounds__(kGnThreads, 2)
     k_gn_bwd_sums(const GnParams p, const __grid_constant__ SeqPlan plan) {
   extern __shared__ float sm[];  // [TY][C] A, then [TY][C] B
+  using S = Span<V, GS>;
+  grid_release();
   const int nvec = p.c / V;
   const Place at(nvec);
   const Chunk ch(plan, blockIdx.x, p.chunk);
@@ -296,50 +422,42 @@ __global__ void __launch_bounds__(kGnThreads)
   const float* stats = p.stats + static_cast<int64_t>(ch.seq) * p.groups * 2;
   if (at.live) {
     for (int cv = at.tx; cv < nvec; cv += at.TX) {
-      float mean[V], rstd[V], w[V], b[V], sa[V], sb[V];
+      F2 mean[S::NR], rstd[S::NR], w[S::NP], b[S::NP], sa[S::NP], sb[S::NP];
+      S::load(stats, 2, cv * V, p.cg, mean);
+      S::load(stats + 1, 2, cv * V, p.cg, rstd);
 #pragma unroll
-      for (int e = 0; e < V; ++e) {
-        const int c = cv * V + e, g = c / p.cg;
-        mean[e] = stats[2 * g];
-        rstd[e] = stats[2 * g + 1];
-        w[e] = load_w(p.w, p.wdtype, c, 1.f);
-        b[e] = load_w(p.b, p.wdtype, c, 0.f);
-        sa[e] = sb[e] = 0.f;
+      for (int i = 0; i < S::NP; ++i) {
+        const int c = cv * V + 2 * i, d = V > 1 ? c + 1 : c;
+        w[i] = f2(load_w(p.w, p.wdtype, c, 1.f), load_w(p.w, p.wdtype, d, 1.f));
+        b[i] = f2(load_w(p.b, p.wdtype, c, 0.f), load_w(p.b, p.wdtype, d, 0.f));
+        sa[i] = sb[i] = 0ull;
       }
       const T* px = x + ch.row0 * p.xs + cv * V;
       const T* pd = dy + ch.row0 * p.c + cv * V;
-      auto add = [&](const Pack<T, V>& v, const Pack<T, V>& d) {
+      Pack<T, V> v[2], g[2];
+      for_rows<2>(
+          ch.rows, at,
+          [&](int u, int r) {
+            v[u].load(px + static_cast<int64_t>(r) * p.xs);
+            g[u].load(pd + static_cast<int64_t>(r) * p.c);
+          },
+          [&](int u, int) {
 #pragma unroll
-        for (int e = 0; e < V; ++e) {
-          float xhat;
-          const float dz = gn_dz(Cvt<T>::to_f(v.t[e]), Cvt<T>::to_f(d.t[e]), mean[e], rstd[e], w[e], b[e], p.silu,
-                                 xhat);
-          sa[e] += dz;
-          sb[e] = fmaf(dz, xhat, sb[e]);
-        }
-      };
-      constexpr int U = 2;
-      int r = at.ty;
-      for (; r + (U - 1) * at.TY < ch.rows; r += U * at.TY) {
-        Pack<T, V> v[U], d[U];
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-          v[u].load(px + static_cast<int64_t>(r + u * at.TY) * p.xs);
-          d[u].load(pd + static_cast<int64_t>(r + u * at.TY) * p.c);
-        }
-#pragma unroll
-        for (int u = 0; u < U; ++u) add(v[u], d[u]);
-      }
-      for (; r < ch.rows; r += at.TY) {
-        Pack<T, V> v, d;
-        v.load(px + static_cast<int64_t>(r) * p.xs);
-        d.load(pd + static_cast<int64_t>(r) * p.c);
-        add(v, d);
-      }
+            for (int i = 0; i < S::NP; ++i) {
+              F2 xhat;
+              const F2 dz = gn_dz(get_pair<T, V>(v[u], i), get_pair<T, V>(g[u], i), mean[S::of(i)], rstd[S::of(i)],
+                                  w[i], b[i], p.silu, xhat);
+              sa[i] = add_f2(sa[i], dz);
+              sb[i] = fma_f2(dz, xhat, sb[i]);
+            }
+          });
 #pragma unroll
       for (int e = 0; e < V; ++e) {
-        s_a[at.ty * p.c + cv * V + e] = sa[e];
-        s_b[at.ty * p.c + cv * V + e] = sb[e];
+        float lo, hi;
+        f2_split(sa[e / 2], lo, hi);
+        s_a[at.ty * p.c + cv * V + e] = e & 1 ? hi : lo;
+        f2_split(sb[e / 2], lo, hi);
+        s_b[at.ty * p.c + cv * V + e] = e & 1 ? hi : lo;
       }
     }
   }
@@ -374,14 +492,16 @@ __global__ void __launch_bounds__(kGnThreads)
 
 constexpr int kGnChanBlock = 32;  // channels per dw / db CTA
 
-// CTAs [0, items) write dx; the CTAs behind them sum dw and db over the items.
-template <typename T, int V>
-__global__ void __launch_bounds__(kGnThreads)
-    k_gn_bwd_apply(const GnParams p, const __grid_constant__ SeqPlan plan, int dx_items) {
+// CTAs [0, chan_ctas) sum dw and db over the items; the others write dx.
+template <typename T, int V, int GS>
+__global__ void __launch_bounds__(kGnThreads, 2)
+    k_gn_bwd_apply(const GnParams p, const __grid_constant__ SeqPlan plan, int chan_ctas) {
   extern __shared__ float sm[];
+  using S = Span<V, GS>;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (static_cast<int>(blockIdx.x) >= dx_items) {
-    const int c = (blockIdx.x - dx_items) * kGnChanBlock + lane;
+  grid_wait();
+  if (static_cast<int>(blockIdx.x) < chan_ctas) {
+    const int c = blockIdx.x * kGnChanBlock + lane;
     float a = 0.f, b = 0.f;
     if (c < p.c)
       for (int i = warp; i < p.items; i += kGnWarps) {
@@ -405,7 +525,7 @@ __global__ void __launch_bounds__(kGnThreads)
   }
   float* s_m1 = sm;
   float* s_m2 = sm + p.groups;
-  const int item = dx_items - 1 - blockIdx.x;
+  const int item = p.items - 1 - (blockIdx.x - chan_ctas);
   const Chunk ch(plan, item, p.chunk);
   const float inv_n = 1.f / (static_cast<float>(ch.seq_rows) * p.cg);
   for (int g = warp; g < p.groups; g += kGnWarps) {
@@ -419,8 +539,8 @@ __global__ void __launch_bounds__(kGnThreads)
     a = warp_sum(a);
     b = warp_sum(b);
     if (lane == 0) {
-      s_m1[g] = a * inv_n;
-      s_m2[g] = b * inv_n;
+      s_m1[g] = -a * inv_n;
+      s_m2[g] = -b * inv_n;
     }
   }
   __syncthreads();
@@ -432,49 +552,39 @@ __global__ void __launch_bounds__(kGnThreads)
   T* dx = static_cast<T*>(p.dx);
   const float* stats = p.stats + static_cast<int64_t>(ch.seq) * p.groups * 2;
   for (int cv = at.tx; cv < nvec; cv += at.TX) {
-    float mean[V], rstd[V], w[V], b[V], m1[V], m2[V];
+    F2 mean[S::NR], rstd[S::NR], m1[S::NR], m2[S::NR], w[S::NP], b[S::NP];
+    S::load(stats, 2, cv * V, p.cg, mean);
+    S::load(stats + 1, 2, cv * V, p.cg, rstd);
+    S::load(s_m1, 1, cv * V, p.cg, m1);
+    S::load(s_m2, 1, cv * V, p.cg, m2);
 #pragma unroll
-    for (int e = 0; e < V; ++e) {
-      const int c = cv * V + e, g = c / p.cg;
-      mean[e] = stats[2 * g];
-      rstd[e] = stats[2 * g + 1];
-      w[e] = load_w(p.w, p.wdtype, c, 1.f);
-      b[e] = load_w(p.b, p.wdtype, c, 0.f);
-      m1[e] = s_m1[g];
-      m2[e] = s_m2[g];
+    for (int i = 0; i < S::NP; ++i) {
+      const int c = cv * V + 2 * i, d = V > 1 ? c + 1 : c;
+      w[i] = f2(load_w(p.w, p.wdtype, c, 1.f), load_w(p.w, p.wdtype, d, 1.f));
+      b[i] = f2(load_w(p.b, p.wdtype, c, 0.f), load_w(p.b, p.wdtype, d, 0.f));
     }
     const T* px = x + ch.row0 * p.xs + cv * V;
     const T* pd = dy + ch.row0 * p.c + cv * V;
     T* po = dx + ch.row0 * p.c + cv * V;
-    auto put = [&](const Pack<T, V>& v, const Pack<T, V>& d, int r) {
-      Pack<T, V> o;
+    Pack<T, V> v[2], g[2];
+    for_rows<2>(
+        ch.rows, at,
+        [&](int u, int r) {
+          v[u].load(px + static_cast<int64_t>(r) * p.xs);
+          g[u].load(pd + static_cast<int64_t>(r) * p.c);
+        },
+        [&](int u, int r) {
+          Pack<T, V> o;
 #pragma unroll
-      for (int e = 0; e < V; ++e) {
-        float xhat;
-        const float dz = gn_dz(Cvt<T>::to_f(v.t[e]), Cvt<T>::to_f(d.t[e]), mean[e], rstd[e], w[e], b[e], p.silu,
-                               xhat);
-        o.t[e] = Cvt<T>::from_f(rstd[e] * (fmaf(w[e], dz, -m1[e]) - xhat * m2[e]));
-      }
-      o.store(po + static_cast<int64_t>(r) * p.c);
-    };
-    constexpr int U = 2;
-    int r = at.ty;
-    for (; r + (U - 1) * at.TY < ch.rows; r += U * at.TY) {
-      Pack<T, V> v[U], d[U];
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        v[u].load(px + static_cast<int64_t>(r + u * at.TY) * p.xs);
-        d[u].load(pd + static_cast<int64_t>(r + u * at.TY) * p.c);
-      }
-#pragma unroll
-      for (int u = 0; u < U; ++u) put(v[u], d[u], r + u * at.TY);
-    }
-    for (; r < ch.rows; r += at.TY) {
-      Pack<T, V> v, d;
-      v.load(px + static_cast<int64_t>(r) * p.xs);
-      d.load(pd + static_cast<int64_t>(r) * p.c);
-      put(v, d, r);
-    }
+          for (int i = 0; i < S::NP; ++i) {
+            F2 xhat;
+            const int k = S::of(i);
+            const F2 dz = gn_dz(get_pair<T, V>(v[u], i), get_pair<T, V>(g[u], i), mean[k], rstd[k], w[i], b[i], p.silu,
+                                xhat);
+            put_pair<T, V>(o, i, mul_f2(rstd[k], fma_f2(xhat, m2[k], fma_f2(w[i], dz, m1[k]))));
+          }
+          o.store(po + static_cast<int64_t>(r) * p.c);
+        });
   }
 }
 
@@ -521,28 +631,75 @@ size_t gn_sum_smem(int c, int nvec) {
   return sizeof(float) * 2 * static_cast<size_t>(ty) * c;  // at most 32 KB: TY * C <= 512 * 8 or C <= 4096
 }
 
-template <typename T, int V>
-sc_status gn_forward_v(Handle* h, GnParams p, const int32_t* cu, int batch) {
-  p.chunk = gn_chunk(h, cu[batch], p.c / V);
-  GnCall call;
-  sc_status st = gn_plan(h, cu, batch, p.chunk, &call);
-  if (st != SC_OK) return st;
-  p.items = call.items;
-  cudaError_t e = dev_alloc(h, reinterpret_cast<void**>(&p.part), sizeof(float2) * p.groups * p.items);
-  if (e != cudaSuccess) {
-    dev_free(h, call.table);
-    return cuda_error(h, e, "group norm workspace");
+// Launches `kernel` so that it may start before the stream's kernels before it
+// end; it waits for them itself (grid_wait).  Or with clusters of `ranks`.
+template <typename... P, typename... A>
+cudaError_t launch_ex(Handle* h, void (*kernel)(P...), int grid, size_t smem, int ranks, A... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(grid));
+  cfg.blockDim = dim3(kGnThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = h->stream;
+  cudaLaunchAttribute at[1];
+  if (ranks > 0) {
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = static_cast<unsigned>(ranks);
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  } else {
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
   }
-  h->launches += 2;
-  k_gn_stats<T, V><<<p.items, kGnThreads, gn_sum_smem(p.c, p.c / V), h->stream>>>(p, call.plan);
-  k_gn_apply<T, V><<<p.items, kGnThreads, sizeof(float) * 2 * p.groups, h->stream>>>(p, call.plan);
-  e = cudaGetLastError();
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  ++h->launches;
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
+// Sequences up to this many bytes per CTA of a cluster of eight take one kernel.
+constexpr int64_t kGnClusterBytes = 64 * 1024;
+constexpr int kGnClusterMax = 8;
+
+template <typename T, int V, int GS>
+sc_status gn_forward_v(Handle* h, GnParams p, const int32_t* cu, int batch) {
+  int64_t longest = 0;
+  for (int s = 0; s < batch; ++s) longest = std::max<int64_t>(longest, static_cast<int64_t>(cu[s + 1]) - cu[s]);
+  const int64_t bytes = longest * p.c * static_cast<int64_t>(sizeof(T));
+  const int ty = kGnThreads / std::min(p.c / V, kGnThreads);
+  GnCall call;
+  cudaError_t e;
+  if (bytes <= kGnClusterMax * kGnClusterBytes) {
+    std::vector<SeqRec> recs;
+    for (int s = 0; s < batch; ++s)
+      if (cu[s + 1] > cu[s])
+        recs.push_back(SeqRec{cu[s], cu[s + 1], 0, 0, static_cast<int32_t>(recs.size()), s});
+    sc_status st = make_plan(h, recs, &call.plan, &call.table);
+    if (st != SC_OK) return st;
+    // a rank for every eight rows of a row lane
+    int ranks = 1;
+    while (ranks < kGnClusterMax && longest > 8ll * ty * ranks) ranks *= 2;
+    e = launch_ex(h, k_gn_cluster<T, V, GS>, static_cast<int>(recs.size()) * ranks,
+                  gn_sum_smem(p.c, p.c / V) + sizeof(float) * 4 * p.groups, ranks, p, call.plan, ranks);
+  } else {
+    p.chunk = gn_chunk(h, cu[batch], p.c / V);
+    sc_status st = gn_plan(h, cu, batch, p.chunk, &call);
+    if (st != SC_OK) return st;
+    p.items = call.items;
+    e = dev_alloc(h, reinterpret_cast<void**>(&p.part), sizeof(float2) * p.groups * p.items);
+    if (e != cudaSuccess) {
+      dev_free(h, call.table);
+      return cuda_error(h, e, "group norm workspace");
+    }
+    ++h->launches;
+    k_gn_stats<T, V><<<p.items, kGnThreads, gn_sum_smem(p.c, p.c / V), h->stream>>>(p, call.plan);
+    e = launch_ex(h, k_gn_apply<T, V, GS>, p.items, sizeof(float) * 2 * p.groups, 0, p, call.plan);
+  }
+  if (e == cudaSuccess) e = cudaGetLastError();
   dev_free(h, p.part);
   dev_free(h, call.table);
   return e == cudaSuccess ? SC_OK : cuda_error(h, e, "group norm launch");
 }
 
-template <typename T, int V>
+template <typename T, int V, int GS>
 sc_status gn_backward_v(Handle* h, GnParams p, const int32_t* cu, int batch) {
   p.chunk = gn_chunk(h, cu[batch], p.c / V);
   GnCall call;
@@ -560,28 +717,40 @@ sc_status gn_backward_v(Handle* h, GnParams p, const int32_t* cu, int batch) {
   p.chan = reinterpret_cast<float*>(ws + part);
   const int dx_items = p.dx ? p.items : 0;
   const int chan_ctas = p.dw || p.db ? (p.c + kGnChanBlock - 1) / kGnChanBlock : 0;
-  h->launches += 2;
-  k_gn_bwd_sums<T, V><<<p.items, kGnThreads, gn_sum_smem(p.c, p.c / V), h->stream>>>(p, call.plan);
-  const size_t smem = sizeof(float) * 2 * std::max(p.groups, kGnThreads);
-  k_gn_bwd_apply<T, V><<<dx_items + chan_ctas, kGnThreads, smem, h->stream>>>(p, call.plan, dx_items);
-  e = cudaGetLastError();
+  ++h->launches;
+  k_gn_bwd_sums<T, V, GS><<<p.items, kGnThreads, gn_sum_smem(p.c, p.c / V), h->stream>>>(p, call.plan);
+  e = launch_ex(h, k_gn_bwd_apply<T, V, GS>, dx_items + chan_ctas, sizeof(float) * 2 * std::max(p.groups, kGnThreads), 0,
+                p, call.plan, chan_ctas);
+  if (e == cudaSuccess) e = cudaGetLastError();
   dev_free(h, ws);
   dev_free(h, call.table);
   return e == cudaSuccess ? SC_OK : cuda_error(h, e, "group norm backward launch");
+}
+
+// Channels of a vector that share a group: the whole vector, four of eight, or
+// each its own.  Eight channels with statistics of their own spill registers:
+// such rows go by vectors of four.
+template <typename T, int V>
+sc_status gn_run(Handle* h, const GnParams& p, const int32_t* cu, int batch, bool backward) {
+  if constexpr (V >= 4)
+    if (p.cg % V == 0) return backward ? gn_backward_v<T, V, V>(h, p, cu, batch) : gn_forward_v<T, V, V>(h, p, cu, batch);
+  if constexpr (V == 8) {
+    if (p.cg % 4 == 0) return backward ? gn_backward_v<T, V, 4>(h, p, cu, batch) : gn_forward_v<T, V, 4>(h, p, cu, batch);
+    return gn_run<T, 4>(h, p, cu, batch, backward);
+  } else {
+    return backward ? gn_backward_v<T, V, 1>(h, p, cu, batch) : gn_forward_v<T, V, 1>(h, p, cu, batch);
+  }
 }
 
 template <typename T>
 sc_status gn_dispatch(Handle* h, const GnParams& p, const int32_t* cu, int batch, bool backward) {
   const void* ptrs[4] = {p.x, backward ? p.dy : p.y, backward ? p.dx : p.y, nullptr};
   const int v = gn_vec<T>(p.c, p.xs, ptrs, 3);
-  switch (v) {
-    case 8:
-      if constexpr (sizeof(T) == 2) return backward ? gn_backward_v<T, 8>(h, p, cu, batch) : gn_forward_v<T, 8>(h, p, cu, batch);
-      [[fallthrough]];
-    case 4: return backward ? gn_backward_v<T, 4>(h, p, cu, batch) : gn_forward_v<T, 4>(h, p, cu, batch);
-    case 2: return backward ? gn_backward_v<T, 2>(h, p, cu, batch) : gn_forward_v<T, 2>(h, p, cu, batch);
-    default: return backward ? gn_backward_v<T, 1>(h, p, cu, batch) : gn_forward_v<T, 1>(h, p, cu, batch);
-  }
+  if constexpr (sizeof(T) == 2)
+    if (v == 8) return gn_run<T, 8>(h, p, cu, batch, backward);
+  if (v == 4) return gn_run<T, 4>(h, p, cu, batch, backward);
+  if (v == 2) return gn_run<T, 2>(h, p, cu, batch, backward);
+  return gn_run<T, 1>(h, p, cu, batch, backward);
 }
 
 }  // namespace

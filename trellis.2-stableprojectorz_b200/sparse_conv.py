@@ -81,8 +81,10 @@ class Engine:
     def call(self, name, *args):
         """One library call on torch's current stream of this device, safe from any thread."""
         with self._op_lock:
-            self.lib.sc_set_stream(self._op_handle, torch.cuda.current_stream(self.device).cuda_stream)
-            L.check(getattr(self.lib, name)(self._op_handle, *args), self._op_handle, name)
+            self.lib.sc_set_stream(self._op_handle, torch._C._cuda_getCurrentRawStream(self.device.index))
+            st = getattr(self.lib, name)(self._op_handle, *args)
+            if st != L.SC_OK:
+                L.check(st, self._op_handle, name)
 
     def set_conv_ctas(self, max_ctas=0):
         """CTAs of the persistent conv (0 = one per SM); fewer leave SMs for a concurrent collective."""
