@@ -28,12 +28,11 @@ __all__ = ["sparse_group_norm", "sparse_diff_attention"]
 
 def _offsets(cu, rows, name):
     """``cu`` as a ctypes int32 array; it must end at ``rows``."""
-    if isinstance(cu, torch.Tensor):
-        if cu.dim() != 1 or cu.is_floating_point() or cu.dtype == torch.bool:
+    if not isinstance(cu, (list, tuple)):
+        if isinstance(cu, torch.Tensor) and (cu.dim() != 1 or cu.is_floating_point() or cu.dtype == torch.bool):
             raise ValueError(f"{name} must be 1-D whole numbers")
-    if hasattr(cu, "tolist"):
-        cu = cu.tolist()
-    cu = [operator.index(v) for v in cu]
+        cu = cu.tolist() if hasattr(cu, "tolist") else list(cu)
+    cu = list(map(operator.index, cu))
     if len(cu) < 2:
         raise ValueError(f"{name} must be 1-D with batch + 1 entries")
     if cu[-1] != rows:
@@ -45,14 +44,19 @@ def _offsets(cu, rows, name):
     return (ctypes.c_int32 * len(cu))(*cu)
 
 
-def _same_device(x, **others):
-    for name, t in others.items():
+def _same_device(x, *others):
+    for t in others:
         if t is not None and t.device != x.device:
-            raise ValueError(f"{name} is on {t.device}, not on {x.device}")
+            raise ValueError(f"tensors on {x.device} and on {t.device}")
 
 
 def _p(t):
     return None if t is None else t.data_ptr()
+
+
+def _dense(t):
+    """An uninitialised dense tensor like ``t``."""
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
 
 
 def _overlap(a, b):
@@ -87,7 +91,7 @@ def _rows_view(x):
 def _gn_forward(x, groups, weight, bias, eps, cu, silu, out, want_stats):
     x, stride = _rows_view(x)
     wd = _DTYPES[(weight if weight is not None else bias if bias is not None else x).dtype]
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device) if out is None else out
+    y = _dense(x) if out is None else out
     stats = torch.empty((len(cu) - 1, groups, 2), dtype=torch.float32, device=x.device) if want_stats else None
     get_engine(x.device).call("sc_group_norm", _p(x), stride, _p(weight), _p(bias), _p(y), _p(stats), cu, len(cu) - 1,
                               x.shape[1], groups, eps, int(silu), _DTYPES[x.dtype], wd)
@@ -110,9 +114,9 @@ class _GroupNorm(torch.autograd.Function):
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
         x, stride = _rows_view(x)
         dy = dy.contiguous()
-        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need_x else None
-        dw = torch.empty_like(weight, memory_format=torch.contiguous_format) if need_w else None
-        db = torch.empty_like(bias, memory_format=torch.contiguous_format) if need_b else None
+        dx = _dense(x) if need_x else None
+        dw = _dense(weight) if need_w else None
+        db = _dense(bias) if need_b else None
         wd = _DTYPES[(weight if weight is not None else bias if bias is not None else x).dtype]
         weight = None if weight is None else weight.contiguous()
         bias = None if bias is None else bias.contiguous()
@@ -152,7 +156,7 @@ def sparse_group_norm(x, num_groups, weight=None, bias=None, eps=1e-5, cu_seqlen
             raise TypeError(f"{name} must be {x.dtype} or float32")
     if weight is not None and bias is not None and weight.dtype != bias.dtype:
         raise TypeError("weight and bias must have one dtype")
-    _same_device(x, weight=weight, bias=bias)
+    _same_device(x, weight, bias)
     eps = float(eps)
     if not (eps > 0 and math.isfinite(eps)):
         raise ValueError("eps must be positive and finite")
@@ -178,26 +182,28 @@ def sparse_group_norm(x, num_groups, weight=None, bias=None, eps=1e-5, cu_seqlen
 def _tokens(t):
     """``t`` (N, heads, D) with dense tokens 16-byte apart: itself, or a copy."""
     n, h, d = t.shape
-    if t.stride(2) == 1 and (h == 1 or t.stride(1) == d) and t.data_ptr() % 16 == 0:
+    s0, s1, s2 = t.stride()
+    if s2 == 1 and (h == 1 or s1 == d) and t.data_ptr() % 16 == 0:
         if n <= 1:
             return t, h * d
-        if t.stride(0) >= h * d and t.stride(0) % 8 == 0:
-            return t, t.stride(0)
+        if s0 >= h * d and s0 % 8 == 0:
+            return t, s0
     t = t.contiguous()
     return (t if t.data_ptr() % 16 == 0 else t.clone()), h * d
 
 
-def _da_args(q, k, v, lam, cu_q, cu_kv, scale, causal, **more):
+def _da_args(q, k, v, lam, cu_q, cu_kv, scale, causal, out=None, lse=None, maps=None, dout=None,
+             grads=(None, None, None, None)):
     (q, qs), (k, ks), (v, vs) = _tokens(q), _tokens(k), _tokens(v)
-    a = L.ScDiffAttentionArgs(q=_p(q), k=_p(k), v=_p(v), q_stride=qs, k_stride=ks, v_stride=vs,
-                              cu_seqlens_q=ctypes.addressof(cu_q), cu_seqlens_kv=ctypes.addressof(cu_kv),
-                              batch=len(cu_q) - 1, heads=q.shape[1] // 2, kv_heads=v.shape[1], scale=scale,
-                              causal=int(causal), dtype=_DTYPES[q.dtype], **{n: _p(t) for n, t in more.items()})
+    dt, ldt, count, value = _DTYPES[q.dtype], L.SC_F32, 0, 0.0
     if isinstance(lam, torch.Tensor):
         lam = lam.contiguous()
-        a.lam, a.lam_count, a.lam_dtype = _p(lam), lam.numel(), _DTYPES[lam.dtype]
+        ldt, count, at = _DTYPES[lam.dtype], lam.numel(), lam.data_ptr()
     else:
-        a.lam_value, a.lam_dtype = lam, L.SC_F32
+        value, at = lam, None
+    a = L.ScDiffAttentionArgs(q.data_ptr(), k.data_ptr(), v.data_ptr(), at, qs, ks, vs, ctypes.addressof(cu_q),
+                              ctypes.addressof(cu_kv), len(cu_q) - 1, q.shape[1] // 2, v.shape[1], count, value, scale,
+                              causal, dt, ldt, _p(out), _p(lse), _p(maps), _p(dout), *map(_p, grads))
     return a, (q, k, v, lam)  # the tensors the addresses belong to
 
 
@@ -219,12 +225,11 @@ class _DiffAttention(torch.autograd.Function):
     def backward(ctx, dout):
         q, k, v, lam, maps, lse = ctx.saved_tensors
         value, cu_q, cu_kv, scale, causal = ctx.args
-        dense = [torch.empty(t.shape, dtype=t.dtype, device=t.device) if need else None
-                 for t, need in zip((q, k, v, lam), ctx.needs_input_grad)]
+        dense = [_dense(t) if need else None for t, need in zip((q, k, v, lam), ctx.needs_input_grad)]
         dout = dout.contiguous()
         dout = dout if dout.data_ptr() % 16 == 0 else dout.clone()
         a, hold = _da_args(q, k, v, value if lam is None else lam, cu_q, cu_kv, scale, causal, lse=lse,
-                           maps=maps, dout=dout, dq=dense[0], dk=dense[1], dv=dense[2], dlam=dense[3])
+                           maps=maps, dout=dout, grads=dense)
         get_engine(q.device).call("sc_diff_attention_backward", ctypes.byref(a))
         return (*dense, None, None, None, None)
 
@@ -266,10 +271,10 @@ def sparse_diff_attention(q, k, v, lam, cu_seqlens_q, cu_seqlens_kv=None, scale=
             raise ValueError(f"lam must hold 1 or {heads} values")
         if lam.dtype not in (q.dtype, torch.float32):
             raise TypeError(f"lam must be {q.dtype} or float32")
-        _same_device(q, lam=lam)
+        _same_device(q, lam)
     else:
         lam = float(lam)
-    _same_device(q, k=k, v=v)
+    _same_device(q, k, v)
     cu_q = _offsets(cu_seqlens_q, q.shape[0], "cu_seqlens_q")
     if cu_seqlens_kv is None:
         if k.shape[0] != q.shape[0]:

@@ -409,25 +409,46 @@ __global__ void __launch_bounds__(128) k_da_join(const DaFwd p, const __grid_con
   const SeqRec& r = plan.at(rec);
   const int nsplit = max(1, (r.k1 - r.k0 + p.split_keys - 1) / p.split_keys);
   if (nsplit == 1) return;
-  float m1 = -INFINITY, m2 = -INFINITY;
-  for (int s = 0; s < nsplit; ++s) {
-    const float4 ml = p.part_ml[s * p.nq * p.heads + at];
-    m1 = fmaxf(m1, ml.x);
-    m2 = fmaxf(m2, ml.z);
-  }
-  float l1 = 0.f, l2 = 0.f, o1[4] = {}, o2[4] = {};
-  for (int s = 0; s < nsplit; ++s) {
-    const float4 ml = p.part_ml[s * p.nq * p.heads + at];
-    const float* o = p.part_o + (s * p.nq * p.heads + at) * (2 * kDaDv) + 4 * lane;
-    const float w1 = ml.y > 0.f ? exp2f(ml.x - m1) : 0.f, w2 = ml.w > 0.f ? exp2f(ml.z - m2) : 0.f;
-    const float4 a = *reinterpret_cast<const float4*>(o), b = *reinterpret_cast<const float4*>(o + kDaDv);
-    l1 = fmaf(w1, ml.y, l1);
-    l2 = fmaf(w2, ml.w, l2);
-    const float av[4] = {a.x, a.y, a.z, a.w}, bv[4] = {b.x, b.y, b.z, b.w};
+  const int64_t step = p.nq * p.heads;
+  float m1 = -INFINITY, m2 = -INFINITY, l1 = 0.f, l2 = 0.f, o1[4] = {}, o2[4] = {};
+  for (int s0 = 0; s0 < nsplit; s0 += 32) {  // lane = range
+    const int ns = min(32, nsplit - s0);
+    const float4 ml = lane < ns ? p.part_ml[(s0 + lane) * step + at] : make_float4(-INFINITY, 0.f, -INFINITY, 0.f);
+    float t1 = ml.x, t2 = ml.z;
+#pragma unroll
+    for (int x = 16; x > 0; x >>= 1) {
+      t1 = fmaxf(t1, __shfl_xor_sync(0xffffffffu, t1, x));
+      t2 = fmaxf(t2, __shfl_xor_sync(0xffffffffu, t2, x));
+    }
+    const float n1 = fmaxf(m1, t1), n2 = fmaxf(m2, t2);
+    const float a1 = m1 > -INFINITY ? exp2f(m1 - n1) : 0.f, a2 = m2 > -INFINITY ? exp2f(m2 - n2) : 0.f;
+    const float w1 = ml.y > 0.f ? exp2f(ml.x - n1) : 0.f, w2 = ml.w > 0.f ? exp2f(ml.z - n2) : 0.f;
+    float s1 = w1 * ml.y, s2 = w2 * ml.w;
+#pragma unroll
+    for (int x = 16; x > 0; x >>= 1) {
+      s1 += __shfl_xor_sync(0xffffffffu, s1, x);
+      s2 += __shfl_xor_sync(0xffffffffu, s2, x);
+    }
+    l1 = fmaf(l1, a1, s1);
+    l2 = fmaf(l2, a2, s2);
+    m1 = n1;
+    m2 = n2;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      o1[e] = fmaf(w1, av[e], o1[e]);
-      o2[e] = fmaf(w2, bv[e], o2[e]);
+      o1[e] *= a1;
+      o2[e] *= a2;
+    }
+#pragma unroll 4
+    for (int s = 0; s < ns; ++s) {
+      const float* o = p.part_o + ((s0 + s) * step + at) * (2 * kDaDv) + 4 * lane;
+      const float4 a = *reinterpret_cast<const float4*>(o), b = *reinterpret_cast<const float4*>(o + kDaDv);
+      const float u1 = __shfl_sync(0xffffffffu, w1, s), u2 = __shfl_sync(0xffffffffu, w2, s);
+      const float av[4] = {a.x, a.y, a.z, a.w}, bv[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        o1[e] = fmaf(u1, av[e], o1[e]);
+        o2[e] = fmaf(u2, bv[e], o2[e]);
+      }
     }
   }
   const float i1 = l1 > 0.f ? 1.f / l1 : 0.f, i2 = l2 > 0.f ? 1.f / l2 : 0.f, lam = p.lam.get(h);
@@ -486,7 +507,8 @@ sc_status run_forward(Handle* h, const DaArgs& a) {
   p.split_keys = std::max(kTile, (longest + kTile - 1) / kTile * kTile);
   if (tiles < 2 * h->num_sms) {
     const int64_t want = (work + 4ll * h->num_sms - 1) / (4ll * h->num_sms);
-    p.split_keys = static_cast<int>(std::min<int64_t>(p.split_keys, std::max<int64_t>(2, want) * kTile));
+    // four tiles at least: a shorter range costs less than the join
+    p.split_keys = static_cast<int>(std::min<int64_t>(p.split_keys, std::max<int64_t>(4, want) * kTile));
   }
   // the longest first: the tail of the launch is made of short CTAs
   std::stable_sort(recs.begin(), recs.end(),

@@ -40,6 +40,9 @@ namespace {
 constexpr int kGnThreads = 512;
 constexpr int kGnWarps = kGnThreads / 32;
 
+// Rows of a batch of loads (two are in flight, one while the other is used).
+constexpr int kGnStatsBatch = 4, kGnApplyBatch = 2, kGnBwdBatch = 1;
+
 // V consecutive values of T as one aligned load.
 template <int BYTES> struct Word;
 template <> struct Word<16> { using type = uint4; };
@@ -53,7 +56,10 @@ struct Pack {
   union { W w; T t[V]; };
   __device__ __forceinline__ Pack() {}
   __device__ __forceinline__ void load(const T* p) { w = *reinterpret_cast<const W*>(p); }
-  __device__ __forceinline__ void store(T* p) const { *reinterpret_cast<W*>(p) = w; }
+  // last use of a line / a line nobody here reads again: first to leave L2, so
+  // that the rows of the first pass stay for the second
+  __device__ __forceinline__ void load_last(const T* p) { w = __ldcs(reinterpret_cast<const W*>(p)); }
+  __device__ __forceinline__ void store(T* p) const { __stcs(reinterpret_cast<W*>(p), w); }
 };
 
 struct GnParams {
@@ -104,15 +110,16 @@ __device__ __forceinline__ F2 mul_f2(F2 a, F2 b) {
 }
 __device__ __forceinline__ F2 neg_f2(F2 a) { return a ^ 0x8000000080000000ull; }
 
-// 1 / (1 + e^-z) of a pair; e^-z overflowing gives 0
+// 1 / (1 + e^-z) of a pair, with one reciprocal for both: the special function
+// unit is what this arithmetic waits for.  e^-z is cut at 2^60, so that the
+// product of both denominators stays finite (sigmoid >= 2^-60).
 __device__ __forceinline__ F2 sigmoid_f2(F2 z) {
   float a, b;
   f2_split(mul_f2(z, f2(-1.4426950408889634f, -1.4426950408889634f)), a, b);
-  f2_split(add_f2(f2(ex2_ftz(a), ex2_ftz(b)), f2(1.f, 1.f)), a, b);
-  float ra, rb;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(ra) : "f"(a));
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(rb) : "f"(b));
-  return f2(ra, rb);
+  f2_split(add_f2(f2(ex2_ftz(fminf(a, 60.f)), ex2_ftz(fminf(b, 60.f))), f2(1.f, 1.f)), a, b);
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(a * b));
+  return mul_f2(f2(r, r), f2(b, a));
 }
 
 // Pair i of a vector (the last of an odd vector twice) / a pair back into it.
@@ -193,20 +200,22 @@ struct Chunk {
 __device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void grid_release() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
-// Calls f(column vector, first row pointer offsets) ... rows of the chunk in
-// batches of U loads: load(u, row) for each of a batch, then use(u, row).
+// The thread's rows of the chunk in batches of U, the loads of a batch ahead of
+// the use of the one before: load(k, row) into slot k of 2 U, use(k, row).
 template <int U, typename L, typename F>
 __device__ __forceinline__ void for_rows(int rows, const Place& at, L&& load, F&& use) {
-  int r = at.ty;
-  for (; r + (U - 1) * at.TY < rows; r += U * at.TY) {
+  const int step = U * at.TY;
+  auto all = [&](int base, int r, auto&& f) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) load(u, r + u * at.TY);
-#pragma unroll
-    for (int u = 0; u < U; ++u) use(u, r + u * at.TY);
-  }
-  for (; r < rows; r += at.TY) {
-    load(0, r);
-    use(0, r);
+    for (int u = 0; u < U; ++u)
+      if (r + u * at.TY < rows) f(base + u, r + u * at.TY);
+  };
+  all(0, at.ty, load);
+  for (int r = at.ty; r < rows; r += 2 * step) {
+    all(U, r + step, load);
+    all(0, r, use);
+    all(0, r + 2 * step, load);
+    all(U, r + step, use);
   }
 }
 
@@ -223,30 +232,30 @@ __device__ __forceinline__ void gn_chunk_stats(const GnParams& p, const Chunk& c
   const T* x = static_cast<const T*>(p.x);
   if (at.live) {
     for (int cv = at.tx; cv < nvec; cv += at.TX) {
-      F2 mean[NP], m2[NP];
+      F2 nmean[NP], m2[NP];  // the running means, negated
 #pragma unroll
-      for (int i = 0; i < NP; ++i) mean[i] = m2[i] = 0ull;
+      for (int i = 0; i < NP; ++i) nmean[i] = m2[i] = 0ull;
       const T* px = x + ch.row0 * p.xs + cv * V;
       float n = 0.f;
-      Pack<T, V> v[4];
-      for_rows<4>(
+      Pack<T, V> v[2 * kGnStatsBatch];
+      for_rows<kGnStatsBatch>(
           ch.rows, at, [&](int u, int r) { v[u].load(px + static_cast<int64_t>(r) * p.xs); },
           [&](int u, int) {
             n += 1.f;
-            const float inv = __fdividef(1.f, n);
-            const F2 inv2 = f2(inv, inv);
+            const float ninv = __fdividef(-1.f, n);
+            const F2 ninv2 = f2(ninv, ninv);
 #pragma unroll
             for (int i = 0; i < NP; ++i) {
-              const F2 f = get_pair<T, V>(v[u], i), d = add_f2(f, neg_f2(mean[i]));
-              mean[i] = fma_f2(d, inv2, mean[i]);
-              m2[i] = fma_f2(d, add_f2(f, neg_f2(mean[i])), m2[i]);
+              const F2 f = get_pair<T, V>(v[u], i), d = add_f2(f, nmean[i]);
+              nmean[i] = fma_f2(d, ninv2, nmean[i]);
+              m2[i] = fma_f2(d, add_f2(f, nmean[i]), m2[i]);
             }
           });
 #pragma unroll
       for (int e = 0; e < V; ++e) {
         float a, b;
-        f2_split(mean[e / 2], a, b);
-        s_mean[at.ty * p.c + cv * V + e] = e & 1 ? b : a;
+        f2_split(nmean[e / 2], a, b);
+        s_mean[at.ty * p.c + cv * V + e] = e & 1 ? -b : -a;
         f2_split(m2[e / 2], a, b);
         s_m2[at.ty * p.c + cv * V + e] = e & 1 ? b : a;
       }
@@ -284,8 +293,10 @@ __device__ __forceinline__ void gn_chunk_apply(const GnParams& p, const Chunk& c
   const T* x = static_cast<const T*>(p.x);
   T* y = static_cast<T*>(p.y);
   for (int cv = at.tx; cv < nvec; cv += at.TX) {
-    F2 mean[S::NR], a[S::NP], b[S::NP];
-    S::load(s_mean, 1, cv * V, p.cg, mean);
+    F2 nmean[S::NR], a[S::NP], b[S::NP];
+    S::load(s_mean, 1, cv * V, p.cg, nmean);
+#pragma unroll
+    for (int r = 0; r < S::NR; ++r) nmean[r] = neg_f2(nmean[r]);
     {
       F2 rstd[S::NR];
       S::load(s_rstd, 1, cv * V, p.cg, rstd);
@@ -298,14 +309,14 @@ __device__ __forceinline__ void gn_chunk_apply(const GnParams& p, const Chunk& c
     }
     const T* px = x + ch.row0 * p.xs + cv * V;
     T* py = y + ch.row0 * p.c + cv * V;
-    Pack<T, V> v[4];
-    for_rows<4>(
-        ch.rows, at, [&](int u, int r) { v[u].load(px + static_cast<int64_t>(r) * p.xs); },
+    Pack<T, V> v[2 * kGnApplyBatch];
+    for_rows<kGnApplyBatch>(
+        ch.rows, at, [&](int u, int r) { v[u].load_last(px + static_cast<int64_t>(r) * p.xs); },
         [&](int u, int r) {
           Pack<T, V> o;
 #pragma unroll
           for (int i = 0; i < S::NP; ++i) {
-            F2 z = fma_f2(add_f2(get_pair<T, V>(v[u], i), neg_f2(mean[S::of(i)])), a[i], b[i]);
+            F2 z = fma_f2(add_f2(get_pair<T, V>(v[u], i), nmean[S::of(i)]), a[i], b[i]);
             if (p.silu) z = mul_f2(z, sigmoid_f2(z));
             put_pair<T, V>(o, i, z);
           }
@@ -399,11 +410,11 @@ __global__ void __launch_bounds__(kGnThreads, 2)
 }
 
 // dz of a pair: x -> xhat, and the gradient through the activation.
-__device__ __forceinline__ F2 gn_dz(F2 x, F2 dy, F2 mean, F2 rstd, F2 w, F2 b, int silu, F2& xhat) {
-  xhat = mul_f2(add_f2(x, neg_f2(mean)), rstd);
+__device__ __forceinline__ F2 gn_dz(F2 x, F2 dy, F2 nmean, F2 rstd, F2 w, F2 b, int silu, F2& xhat) {
+  xhat = mul_f2(add_f2(x, nmean), rstd);
   if (!silu) return dy;
   const F2 one = f2(1.f, 1.f), z = fma_f2(xhat, w, b), s = sigmoid_f2(z);
-  return mul_f2(mul_f2(dy, s), fma_f2(z, add_f2(one, neg_f2(s)), one));
+  return mul_f2(mul_f2(dy, s), fma_f2(z, fma_f2(s, f2(-1.f, -1.f), one), one));
 }
 
 template <typename T, int V, int GS>
@@ -422,8 +433,10 @@ __global__ void __launch_bounds__(kGnThreads, 2)
   const float* stats = p.stats + static_cast<int64_t>(ch.seq) * p.groups * 2;
   if (at.live) {
     for (int cv = at.tx; cv < nvec; cv += at.TX) {
-      F2 mean[S::NR], rstd[S::NR], w[S::NP], b[S::NP], sa[S::NP], sb[S::NP];
-      S::load(stats, 2, cv * V, p.cg, mean);
+      F2 nmean[S::NR], rstd[S::NR], w[S::NP], b[S::NP], sa[S::NP], sb[S::NP];
+      S::load(stats, 2, cv * V, p.cg, nmean);
+#pragma unroll
+    for (int r = 0; r < S::NR; ++r) nmean[r] = neg_f2(nmean[r]);
       S::load(stats + 1, 2, cv * V, p.cg, rstd);
 #pragma unroll
       for (int i = 0; i < S::NP; ++i) {
@@ -434,8 +447,8 @@ __global__ void __launch_bounds__(kGnThreads, 2)
       }
       const T* px = x + ch.row0 * p.xs + cv * V;
       const T* pd = dy + ch.row0 * p.c + cv * V;
-      Pack<T, V> v[2], g[2];
-      for_rows<2>(
+      Pack<T, V> v[2 * kGnBwdBatch], g[2 * kGnBwdBatch];
+      for_rows<kGnBwdBatch>(
           ch.rows, at,
           [&](int u, int r) {
             v[u].load(px + static_cast<int64_t>(r) * p.xs);
@@ -445,7 +458,7 @@ __global__ void __launch_bounds__(kGnThreads, 2)
 #pragma unroll
             for (int i = 0; i < S::NP; ++i) {
               F2 xhat;
-              const F2 dz = gn_dz(get_pair<T, V>(v[u], i), get_pair<T, V>(g[u], i), mean[S::of(i)], rstd[S::of(i)],
+              const F2 dz = gn_dz(get_pair<T, V>(v[u], i), get_pair<T, V>(g[u], i), nmean[S::of(i)], rstd[S::of(i)],
                                   w[i], b[i], p.silu, xhat);
               sa[i] = add_f2(sa[i], dz);
               sb[i] = fma_f2(dz, xhat, sb[i]);
@@ -552,8 +565,10 @@ __global__ void __launch_bounds__(kGnThreads, 2)
   T* dx = static_cast<T*>(p.dx);
   const float* stats = p.stats + static_cast<int64_t>(ch.seq) * p.groups * 2;
   for (int cv = at.tx; cv < nvec; cv += at.TX) {
-    F2 mean[S::NR], rstd[S::NR], m1[S::NR], m2[S::NR], w[S::NP], b[S::NP];
-    S::load(stats, 2, cv * V, p.cg, mean);
+    F2 nmean[S::NR], rstd[S::NR], m1[S::NR], m2[S::NR], w[S::NP], b[S::NP];
+    S::load(stats, 2, cv * V, p.cg, nmean);
+#pragma unroll
+    for (int r = 0; r < S::NR; ++r) nmean[r] = neg_f2(nmean[r]);
     S::load(stats + 1, 2, cv * V, p.cg, rstd);
     S::load(s_m1, 1, cv * V, p.cg, m1);
     S::load(s_m2, 1, cv * V, p.cg, m2);
@@ -566,12 +581,12 @@ __global__ void __launch_bounds__(kGnThreads, 2)
     const T* px = x + ch.row0 * p.xs + cv * V;
     const T* pd = dy + ch.row0 * p.c + cv * V;
     T* po = dx + ch.row0 * p.c + cv * V;
-    Pack<T, V> v[2], g[2];
-    for_rows<2>(
+    Pack<T, V> v[2 * kGnBwdBatch], g[2 * kGnBwdBatch];
+    for_rows<kGnBwdBatch>(
         ch.rows, at,
         [&](int u, int r) {
-          v[u].load(px + static_cast<int64_t>(r) * p.xs);
-          g[u].load(pd + static_cast<int64_t>(r) * p.c);
+          v[u].load_last(px + static_cast<int64_t>(r) * p.xs);
+          g[u].load_last(pd + static_cast<int64_t>(r) * p.c);
         },
         [&](int u, int r) {
           Pack<T, V> o;
@@ -579,7 +594,7 @@ __global__ void __launch_bounds__(kGnThreads, 2)
           for (int i = 0; i < S::NP; ++i) {
             F2 xhat;
             const int k = S::of(i);
-            const F2 dz = gn_dz(get_pair<T, V>(v[u], i), get_pair<T, V>(g[u], i), mean[k], rstd[k], w[i], b[i], p.silu,
+            const F2 dz = gn_dz(get_pair<T, V>(v[u], i), get_pair<T, V>(g[u], i), nmean[k], rstd[k], w[i], b[i], p.silu,
                                 xhat);
             put_pair<T, V>(o, i, mul_f2(rstd[k], fma_f2(xhat, m2[k], fma_f2(w[i], dz, m1[k]))));
           }
@@ -588,12 +603,22 @@ __global__ void __launch_bounds__(kGnThreads, 2)
   }
 }
 
-// Rows per chunk: about two CTAs' worth of chunks per SM, and at least four
-// rows per row lane.
-int gn_chunk(const Handle* h, int64_t rows, int nvec) {
+// Rows per chunk: two CTAs per SM in one wave (a chunk more would be a second
+// one), and at least four rows per row lane.
+int gn_chunk(const Handle* h, const int32_t* cu, int batch, int nvec) {
   const int ty = kGnThreads / std::min(nvec, kGnThreads);
-  const int64_t want = (rows + 2ll * h->num_sms - 1) / (2ll * h->num_sms);
-  return static_cast<int>(std::max<int64_t>(want, 4ll * ty));
+  const int64_t slots = 2ll * h->num_sms;
+  int64_t chunk = std::max<int64_t>((cu[batch] + slots - 1) / slots, 4ll * ty);
+  for (int tries = 0; tries < 16; ++tries, chunk += (chunk + 63) / 64) {
+    int64_t items = 0, seqs = 0;
+    for (int s = 0; s < batch; ++s) {
+      const int64_t len = static_cast<int64_t>(cu[s + 1]) - cu[s];
+      items += (len + chunk - 1) / chunk;
+      seqs += len > 0;
+    }
+    if (items <= slots || seqs > slots / 2) break;
+  }
+  return static_cast<int>(std::min<int64_t>(chunk, 0x7fffffff));
 }
 
 struct GnCall {
@@ -680,7 +705,7 @@ sc_status gn_forward_v(Handle* h, GnParams p, const int32_t* cu, int batch) {
     e = launch_ex(h, k_gn_cluster<T, V, GS>, static_cast<int>(recs.size()) * ranks,
                   gn_sum_smem(p.c, p.c / V) + sizeof(float) * 4 * p.groups, ranks, p, call.plan, ranks);
   } else {
-    p.chunk = gn_chunk(h, cu[batch], p.c / V);
+    p.chunk = gn_chunk(h, cu, batch, p.c / V);
     sc_status st = gn_plan(h, cu, batch, p.chunk, &call);
     if (st != SC_OK) return st;
     p.items = call.items;
@@ -701,7 +726,7 @@ sc_status gn_forward_v(Handle* h, GnParams p, const int32_t* cu, int batch) {
 
 template <typename T, int V, int GS>
 sc_status gn_backward_v(Handle* h, GnParams p, const int32_t* cu, int batch) {
-  p.chunk = gn_chunk(h, cu[batch], p.c / V);
+  p.chunk = gn_chunk(h, cu, batch, p.c / V);
   GnCall call;
   sc_status st = gn_plan(h, cu, batch, p.chunk, &call);
   if (st != SC_OK) return st;

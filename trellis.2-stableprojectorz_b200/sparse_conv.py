@@ -115,6 +115,9 @@ def get_engine(device=None, map_mode="hash"):
     dev = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
     idx = dev.index if dev.index is not None else torch.cuda.current_device()
     key = (idx, map_mode)
+    eng = _engines.get(key)
+    if eng is not None:
+        return eng
     with _engines_lock:
         if key not in _engines:
             _engines[key] = Engine(torch.device("cuda", idx), map_mode)
