@@ -236,27 +236,23 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int limit = live ? min(tile.key1, key_limit(rec, tok, p.causal)) : 0;
     float mx = -INFINITY, l = 0.f;
     bool ok = nk > 0;
-    auto wait_warp = [&](uint32_t bar, uint32_t parity) -> bool {
-      int w = 1;
-      if (lane == 0) w = mbar_wait(bar, parity, p.err) ? 1 : 0;
-      return __shfl_sync(0xffffffffu, w, 0) != 0;
-    };
     if ((warp & 3) * 32 < rows) {
       const int least = __reduce_min_sync(0xffffffffu, live ? limit : 0x7fffffff);
       for (int j = 0; j < nk; ++j) {
         const int valid = limit - (tile.key0 + j * kTile);  // this row sees the first `valid` columns
         const bool full = least - (tile.key0 + j * kTile) >= kTile;
-        if (!wait_warp(s_full0 + 8u * m, j & 1)) {
+        if (!warp_wait(s_full0 + 8u * m, j & 1, p.err)) {
           ok = false;
           break;
         }
         tc_fence_after();
         float s[2][64];
-        tmem_ld64(lane_base, s[0]);
-        tmem_ld64(lane_base + 64u, s[1]);
+        tmem_ld64x2(lane_base, lane_base + 64u, s[0], s[1]);
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(s_free);
+        // asked for here, looked at behind the maximum
+        const bool o_ready = j == 0 || mbar_try_wait(o_done0 + 8u * m, (j - 1) & 1);
         if (!full) {
 #pragma unroll
           for (int i = 0; i < kTile; ++i) s[i / 64][i % 64] = i < valid ? s[i / 64][i % 64] : -INFINITY;  // 2^-inf = 0
@@ -273,7 +269,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const float alpha = move ? ex2_ftz(mx - m_new) : 1.f;
         // the product of this map's last step: O_m is complete and P_m is read
         if (j > 0) {
-          if (!wait_warp(o_done0 + 8u * m, (j - 1) & 1)) {
+          if (!__all_sync(0xffffffffu, o_ready) && !warp_wait(o_done0 + 8u * m, (j - 1) & 1, p.err)) {
             ok = false;
             break;
           }
@@ -317,7 +313,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         l = fmaf(l, alpha, a + b);
         mx = m_new;
       }
-      ok = ok && wait_warp(o_done0 + 8u * m, (nk - 1) & 1);
+      ok = ok && warp_wait(o_done0 + 8u * m, (nk - 1) & 1, p.err);
       // the last product of a map is issued after every score product, so Q's
       // shared memory is free (warps without rows come here at once: they may not write)
       s_row[m * kTile + row] = make_float2(ok ? mx : -INFINITY, ok ? l : 0.f);

@@ -364,11 +364,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         nd[m] = p.st[(2 + m) * static_cast<int64_t>(p.heads) * p.np + at];
       }
     bool ok = true;
-    auto wait_warp = [&](uint32_t bar, uint32_t parity) -> bool {
-      int w = 1;
-      if (lane == 0) w = mbar_wait(bar, parity, p.err) ? 1 : 0;
-      return __shfl_sync(0xffffffffu, w, 0) != 0;
-    };
     const unsigned long long sc2 = f2(p.scale_log2, p.scale_log2);
     // tile and head of the group's step, its place in the ring
     int ty = n > 0 ? (t0 + grp) % ny : 0, head = KV ? g * p.rep + (n > 0 ? (t0 + grp) / ny : 0) : blockIdx.y;
@@ -388,14 +383,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint32_t turn = (j >> 1) & 1;
       const bool full = c0 >= lo_max && c0 + kY <= hi_min;
       const float4* st = reinterpret_cast<const float4*>(smem + kOffY + place * C::kStage + 4 * kYBytes);
-      ok = wait_warp(s_full0 + 8u * grp, turn);
+      ok = warp_wait(s_full0 + 8u * grp, turn, p.err);
       // the statistics landed with the tile: the MMA thread has seen that, this one has not
-      if (KV) ok = ok && wait_warp(y_full0 + 8 * place, use);
+      if (KV) ok = ok && warp_wait(y_full0 + 8 * place, use, p.err);
       if (!ok) break;
       tc_fence_after();
       float w[2][kY], dp[kY];
-#pragma unroll
-      for (int m = 0; m < 2; ++m) tmem_ld48(lane_base + C::kS + kY * m, w[m]);
+      tmem_ld48x2(lane_base + C::kS, lane_base + C::kS + kY, w[0], w[1]);
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(s_free);
@@ -414,13 +408,15 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       };
       weights(0);
-      ok = wait_warp(dp_full0 + 8u * grp, turn);
+      ok = warp_wait(dp_full0 + 8u * grp, turn, p.err);
       if (!ok) break;
       tc_fence_after();
       tmem_ld48(lane_base + C::kDp, dp);
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(dp_free);
+      // asked for here, looked at when the results are ready to be stored
+      const bool p_ready = j == 0 || mbar_try_wait(p_free0 + 8u * (grp ^ 1), ((j - 1) >> 1) & 1);
       weights(1);
       if (!full) {  // weight 0, and 0 * NaN of a row that is not seen
 #pragma unroll
@@ -472,7 +468,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       // the columns of the step before are read: only these stores and the
       // products stand between one step's wait here and the next one's
-      if (j > 0) ok = wait_warp(p_free0 + 8u * (grp ^ 1), ((j - 1) >> 1) & 1);
+      if (!__all_sync(0xffffffffu, p_ready)) ok = warp_wait(p_free0 + 8u * (grp ^ 1), ((j - 1) >> 1) & 1, p.err);
       if (!ok) break;
       tc_fence_after();
 #pragma unroll
@@ -486,7 +482,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(ds_full);
     }
-    ok = ok && n > 0 && wait_warp(done_bar, 0);
+    ok = ok && n > 0 && warp_wait(done_bar, 0, p.err);
     tc_fence_after();
     // group 0 writes dX_1, group 1 dX_2, and each its half of dV's columns
     const int xheads = KV ? p.kv_heads : p.heads;
