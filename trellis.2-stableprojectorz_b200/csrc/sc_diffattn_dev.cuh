@@ -186,8 +186,8 @@ __device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&v)[8])
 }
 
 // Register split of a 384-thread block launched with 168 registers a thread:
-// warps 0-3 keep 88, warps 4-11 take 208 (128 * 88 + 256 * 208 = 384 * 168).
-__device__ __forceinline__ void regs_release() { asm volatile("setmaxnreg.dec.sync.aligned.u32 88;"); }
-__device__ __forceinline__ void regs_take() { asm volatile("setmaxnreg.inc.sync.aligned.u32 208;"); }
+// warps 0-3 keep 72, warps 4-11 take 216 (128 * 72 + 256 * 216 = 384 * 168).
+__device__ __forceinline__ void regs_release() { asm volatile("setmaxnreg.dec.sync.aligned.u32 72;"); }
+__device__ __forceinline__ void regs_take() { asm volatile("setmaxnreg.inc.sync.aligned.u32 216;"); }
 
 }  // namespace sc

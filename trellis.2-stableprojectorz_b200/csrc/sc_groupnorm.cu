@@ -81,6 +81,7 @@ struct GnParams {
   int items;
   float eps;
   int silu;
+  int* err;
 };
 
 __device__ __forceinline__ float load_w(const void* p, int wdtype, int c, float none) {
@@ -219,9 +220,72 @@ __device__ __forceinline__ void for_rows(int rows, const Place& at, L&& load, F&
   }
 }
 
+// The same rows through shared memory: blocks of 2 TY consecutive rows (at most
+// 16 KB; of two arrays: TY rows each) arrive by bulk copies in a ring of six, so
+// the bytes in flight cost no registers: 96 KB a CTA.  Dense rows of 16-byte
+// vectors only.  `last_first` walks the chunk's blocks from its end: the rows
+// that the pass before read last are the ones still in L2.  use(pack of array 0,
+// pack of array 1, row).
+constexpr int kGnRing = 6, kGnBlock = 16 * 1024, kGnRingSmem = kGnRing * kGnBlock + 16 * kGnRing + 128;
+template <int ARRAYS, typename T, int V, typename F>
+__device__ __forceinline__ void ring_rows(const GnParams& p, const Chunk& ch, const Place& at, float* sm, const void* a0,
+                                          const void* a1, bool last_first, F&& use) {
+  const uint32_t base = (smem_u32(sm) + 127u) & ~127u;
+  uint8_t* ring = reinterpret_cast<uint8_t*>(sm) + (base - smem_u32(sm));
+  const uint32_t full0 = base + kGnRing * kGnBlock, empty0 = full0 + 8 * kGnRing;
+  const int row_bytes = p.c * static_cast<int>(sizeof(T)), per = (2 / ARRAYS) * at.TY;
+  const int blocks = (ch.rows + per - 1) / per;
+  const char* src[2] = {static_cast<const char*>(a0) + ch.row0 * row_bytes,
+                        static_cast<const char*>(a1) + ch.row0 * row_bytes};
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kGnRing; ++i) {
+      mbar_init(full0 + 8 * i, 1);
+      mbar_init(empty0 + 8 * i, kGnWarps);
+    }
+    fence_mbar_init();
+  }
+  __syncthreads();
+  auto issue = [&](int k) {
+    const int b = last_first ? blocks - 1 - k : k, s = k % kGnRing;
+    const uint32_t bytes = static_cast<uint32_t>(min(per, ch.rows - b * per)) * row_bytes;
+    mbar_arrive_expect_tx(full0 + 8 * s, ARRAYS * bytes);
+    for (int i = 0; i < ARRAYS; ++i)
+      bulk_load(base + s * kGnBlock + i * (kGnBlock / 2), src[i] + static_cast<int64_t>(b) * per * row_bytes, bytes,
+                full0 + 8 * s);
+  };
+  if (threadIdx.x == 0)
+    for (int k = 0; k < min(blocks, kGnRing - 1); ++k) issue(k);
+  int s = 0, turn = 0;
+  for (int k = 0; k < blocks; ++k) {
+    if (threadIdx.x == 0 && k + kGnRing - 1 < blocks) {
+      // the slot of block k - 1, once every warp has left it
+      if (k == 0 || mbar_wait(empty0 + 8 * ((k - 1) % kGnRing), ((k - 1) / kGnRing) & 1, p.err)) issue(k + kGnRing - 1);
+    }
+    __syncwarp();
+    if (!mbar_wait(full0 + 8 * s, turn, p.err)) break;
+    const int b = last_first ? blocks - 1 - k : k, rows = min(per, ch.rows - b * per);
+    if (at.live) {
+#pragma unroll
+      for (int u = 0; u < 2 / ARRAYS; ++u) {
+        const int r = at.ty + u * at.TY;
+        if (r < rows) {
+          Pack<T, V> v, g;
+          v.load(reinterpret_cast<const T*>(ring + s * kGnBlock + r * row_bytes) + at.tx * V);
+          if (ARRAYS == 2) g.load(reinterpret_cast<const T*>(ring + s * kGnBlock + kGnBlock / 2 + r * row_bytes) + at.tx * V);
+          use(v, g, b * per + r);
+        }
+      }
+    }
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) mbar_arrive(empty0 + 8 * s);
+    if (++s == kGnRing) s = 0, turn ^= 1;
+  }
+  __syncthreads();  // sm may be used again
+}
+
 // (mean, M2) of every group of the chunk, to dst[g * stride].  sm: [TY][C]
 // means, then [TY][C] M2.
-template <typename T, int V>
+template <typename T, int V, bool RING = false>
 __device__ __forceinline__ void gn_chunk_stats(const GnParams& p, const Chunk& ch, float* sm, float2* dst,
                                                int64_t stride) {
   constexpr int NP = (V + 1) / 2;
@@ -230,27 +294,34 @@ __device__ __forceinline__ void gn_chunk_stats(const GnParams& p, const Chunk& c
   float* s_mean = sm;
   float* s_m2 = sm + at.TY * p.c;
   const T* x = static_cast<const T*>(p.x);
-  if (at.live) {
-    for (int cv = at.tx; cv < nvec; cv += at.TX) {
+  if (at.live || RING) {  // the ring's barriers want every thread
+    for (int cv = RING ? min(at.tx, nvec - 1) : at.tx; cv < nvec; cv += RING ? nvec : at.TX) {
       F2 nmean[NP], m2[NP];  // the running means, negated
 #pragma unroll
       for (int i = 0; i < NP; ++i) nmean[i] = m2[i] = 0ull;
       const T* px = x + ch.row0 * p.xs + cv * V;
       float n = 0.f;
-      Pack<T, V> v[2 * kGnStatsBatch];
-      for_rows<kGnStatsBatch>(
-          ch.rows, at, [&](int u, int r) { v[u].load(px + static_cast<int64_t>(r) * p.xs); },
-          [&](int u, int) {
-            n += 1.f;
-            const float ninv = __fdividef(-1.f, n);
-            const F2 ninv2 = f2(ninv, ninv);
+      auto add = [&](const Pack<T, V>& v) {
+        n += 1.f;
+        const float ninv = __fdividef(-1.f, n);
+        const F2 ninv2 = f2(ninv, ninv);
 #pragma unroll
-            for (int i = 0; i < NP; ++i) {
-              const F2 f = get_pair<T, V>(v[u], i), d = add_f2(f, nmean[i]);
-              nmean[i] = fma_f2(d, ninv2, nmean[i]);
-              m2[i] = fma_f2(d, add_f2(f, nmean[i]), m2[i]);
-            }
-          });
+        for (int i = 0; i < NP; ++i) {
+          const F2 f = get_pair<T, V>(v, i), d = add_f2(f, nmean[i]);
+          nmean[i] = fma_f2(d, ninv2, nmean[i]);
+          m2[i] = fma_f2(d, add_f2(f, nmean[i]), m2[i]);
+        }
+      };
+      if constexpr (RING) {
+        ring_rows<1, T, V>(p, ch, at, sm, p.x, nullptr, false,
+                           [&](const Pack<T, V>& v, const Pack<T, V>&, int) { add(v); });
+      } else {
+        Pack<T, V> v[2 * kGnStatsBatch];
+        for_rows<kGnStatsBatch>(
+            ch.rows, at, [&](int u, int r) { v[u].load(px + static_cast<int64_t>(r) * p.xs); },
+            [&](int u, int) { add(v[u]); });
+      }
+      if (at.live)
 #pragma unroll
       for (int e = 0; e < V; ++e) {
         float a, b;
@@ -283,16 +354,16 @@ __device__ __forceinline__ void gn_chunk_stats(const GnParams& p, const Chunk& c
 }
 
 // y of the chunk's rows from s_mean / s_rstd [G].
-template <typename T, int V, int GS>
+template <typename T, int V, int GS, bool RING = false>
 __device__ __forceinline__ void gn_chunk_apply(const GnParams& p, const Chunk& ch, const float* s_mean,
-                                               const float* s_rstd) {
+                                               const float* s_rstd, float* ring = nullptr) {
   using S = Span<V, GS>;
   const int nvec = p.c / V;
   const Place at(nvec);
-  if (!at.live) return;
+  if (!at.live && !RING) return;
   const T* x = static_cast<const T*>(p.x);
   T* y = static_cast<T*>(p.y);
-  for (int cv = at.tx; cv < nvec; cv += at.TX) {
+  for (int cv = RING ? min(at.tx, nvec - 1) : at.tx; cv < nvec; cv += RING ? nvec : at.TX) {
     F2 nmean[S::NR], a[S::NP], b[S::NP];
     S::load(s_mean, 1, cv * V, p.cg, nmean);
 #pragma unroll
@@ -309,29 +380,35 @@ __device__ __forceinline__ void gn_chunk_apply(const GnParams& p, const Chunk& c
     }
     const T* px = x + ch.row0 * p.xs + cv * V;
     T* py = y + ch.row0 * p.c + cv * V;
-    Pack<T, V> v[2 * kGnApplyBatch];
-    for_rows<kGnApplyBatch>(
-        ch.rows, at, [&](int u, int r) { v[u].load_last(px + static_cast<int64_t>(r) * p.xs); },
-        [&](int u, int r) {
-          Pack<T, V> o;
+    auto put = [&](const Pack<T, V>& v, int r) {
+      Pack<T, V> o;
 #pragma unroll
-          for (int i = 0; i < S::NP; ++i) {
-            F2 z = fma_f2(add_f2(get_pair<T, V>(v[u], i), nmean[S::of(i)]), a[i], b[i]);
-            if (p.silu) z = mul_f2(z, sigmoid_f2(z));
-            put_pair<T, V>(o, i, z);
-          }
-          o.store(py + static_cast<int64_t>(r) * p.c);
-        });
+      for (int i = 0; i < S::NP; ++i) {
+        F2 z = fma_f2(add_f2(get_pair<T, V>(v, i), nmean[S::of(i)]), a[i], b[i]);
+        if (p.silu) z = mul_f2(z, sigmoid_f2(z));
+        put_pair<T, V>(o, i, z);
+      }
+      o.store(py + static_cast<int64_t>(r) * p.c);
+    };
+    if constexpr (RING) {
+      ring_rows<1, T, V>(p, ch, at, ring, p.x, nullptr, true,
+                         [&](const Pack<T, V>& v, const Pack<T, V>&, int r) { put(v, r); });
+    } else {
+      Pack<T, V> v[2 * kGnApplyBatch];
+      for_rows<kGnApplyBatch>(
+          ch.rows, at, [&](int u, int r) { v[u].load_last(px + static_cast<int64_t>(r) * p.xs); },
+          [&](int u, int r) { put(v[u], r); });
+    }
   }
 }
 
-template <typename T, int V>
+template <typename T, int V, bool RING>
 __global__ void __launch_bounds__(kGnThreads, 2)
     k_gn_stats(const GnParams p, const __grid_constant__ SeqPlan plan) {
   extern __shared__ float sm[];
   grid_release();
   const Chunk ch(plan, blockIdx.x, p.chunk);
-  gn_chunk_stats<T, V>(p, ch, sm, p.part + blockIdx.x, p.items);
+  gn_chunk_stats<T, V, RING>(p, ch, sm, p.part + blockIdx.x, p.items);
 }
 
 // Mean and rstd of every group of a sequence from its chunks' (mean, M2):
@@ -368,7 +445,7 @@ __device__ __forceinline__ void gn_keep_stats(const GnParams& p, int seq, const 
   }
 }
 
-template <typename T, int V, int GS>
+template <typename T, int V, int GS, bool RING>
 __global__ void __launch_bounds__(kGnThreads, 2)
     k_gn_apply(const GnParams p, const __grid_constant__ SeqPlan plan) {
   extern __shared__ float sm[];
@@ -381,7 +458,7 @@ __global__ void __launch_bounds__(kGnThreads, 2)
              [&](int i, int g) { return p.part[static_cast<int64_t>(g) * p.items + ch.first_item + i]; }, s_mean, s_rstd);
   __syncthreads();
   if (p.stats && item == ch.first_item) gn_keep_stats(p, ch.seq, s_mean, s_rstd);
-  gn_chunk_apply<T, V, GS>(p, ch, s_mean, s_rstd);
+  gn_chunk_apply<T, V, GS, RING>(p, ch, s_mean, s_rstd, s_rstd + p.groups);
 }
 
 // One cluster per sequence (records: one item each); rank r takes the rows
@@ -417,7 +494,7 @@ __device__ __forceinline__ F2 gn_dz(F2 x, F2 dy, F2 nmean, F2 rstd, F2 w, F2 b, 
   return mul_f2(mul_f2(dy, s), fma_f2(z, fma_f2(s, f2(-1.f, -1.f), one), one));
 }
 
-template <typename T, int V, int GS>
+template <typename T, int V, int GS, bool RING>
 __global__ void __launch_bounds__(kGnThreads, 2)
     k_gn_bwd_sums(const GnParams p, const __grid_constant__ SeqPlan plan) {
   extern __shared__ float sm[];  // [TY][C] A, then [TY][C] B
@@ -431,8 +508,8 @@ __global__ void __launch_bounds__(kGnThreads, 2)
   const T* x = static_cast<const T*>(p.x);
   const T* dy = static_cast<const T*>(p.dy);
   const float* stats = p.stats + static_cast<int64_t>(ch.seq) * p.groups * 2;
-  if (at.live) {
-    for (int cv = at.tx; cv < nvec; cv += at.TX) {
+  if (at.live || RING) {
+    for (int cv = RING ? min(at.tx, nvec - 1) : at.tx; cv < nvec; cv += RING ? nvec : at.TX) {
       F2 nmean[S::NR], rstd[S::NR], w[S::NP], b[S::NP], sa[S::NP], sb[S::NP];
       S::load(stats, 2, cv * V, p.cg, nmean);
 #pragma unroll
@@ -447,23 +524,30 @@ __global__ void __launch_bounds__(kGnThreads, 2)
       }
       const T* px = x + ch.row0 * p.xs + cv * V;
       const T* pd = dy + ch.row0 * p.c + cv * V;
-      Pack<T, V> v[2 * kGnBwdBatch], g[2 * kGnBwdBatch];
-      for_rows<kGnBwdBatch>(
-          ch.rows, at,
-          [&](int u, int r) {
-            v[u].load(px + static_cast<int64_t>(r) * p.xs);
-            g[u].load(pd + static_cast<int64_t>(r) * p.c);
-          },
-          [&](int u, int) {
+      auto add = [&](const Pack<T, V>& v, const Pack<T, V>& g) {
 #pragma unroll
-            for (int i = 0; i < S::NP; ++i) {
-              F2 xhat;
-              const F2 dz = gn_dz(get_pair<T, V>(v[u], i), get_pair<T, V>(g[u], i), nmean[S::of(i)], rstd[S::of(i)],
-                                  w[i], b[i], p.silu, xhat);
-              sa[i] = add_f2(sa[i], dz);
-              sb[i] = fma_f2(dz, xhat, sb[i]);
-            }
-          });
+        for (int i = 0; i < S::NP; ++i) {
+          F2 xhat;
+          const F2 dz = gn_dz(get_pair<T, V>(v, i), get_pair<T, V>(g, i), nmean[S::of(i)], rstd[S::of(i)], w[i], b[i],
+                              p.silu, xhat);
+          sa[i] = add_f2(sa[i], dz);
+          sb[i] = fma_f2(dz, xhat, sb[i]);
+        }
+      };
+      if constexpr (RING) {
+        ring_rows<2, T, V>(p, ch, at, sm, p.x, p.dy, false,
+                           [&](const Pack<T, V>& v, const Pack<T, V>& g, int) { add(v, g); });
+      } else {
+        Pack<T, V> v[2 * kGnBwdBatch], g[2 * kGnBwdBatch];
+        for_rows<kGnBwdBatch>(
+            ch.rows, at,
+            [&](int u, int r) {
+              v[u].load(px + static_cast<int64_t>(r) * p.xs);
+              g[u].load(pd + static_cast<int64_t>(r) * p.c);
+            },
+            [&](int u, int) { add(v[u], g[u]); });
+      }
+      if (at.live)
 #pragma unroll
       for (int e = 0; e < V; ++e) {
         float lo, hi;
@@ -506,7 +590,7 @@ __global__ void __launch_bounds__(kGnThreads, 2)
 constexpr int kGnChanBlock = 32;  // channels per dw / db CTA
 
 // CTAs [0, chan_ctas) sum dw and db over the items; the others write dx.
-template <typename T, int V, int GS>
+template <typename T, int V, int GS, bool RING>
 __global__ void __launch_bounds__(kGnThreads, 2)
     k_gn_bwd_apply(const GnParams p, const __grid_constant__ SeqPlan plan, int chan_ctas) {
   extern __shared__ float sm[];
@@ -559,12 +643,12 @@ __global__ void __launch_bounds__(kGnThreads, 2)
   __syncthreads();
   const int nvec = p.c / V;
   const Place at(nvec);
-  if (!at.live) return;
+  if (!at.live && !RING) return;
   const T* x = static_cast<const T*>(p.x);
   const T* dy = static_cast<const T*>(p.dy);
   T* dx = static_cast<T*>(p.dx);
   const float* stats = p.stats + static_cast<int64_t>(ch.seq) * p.groups * 2;
-  for (int cv = at.tx; cv < nvec; cv += at.TX) {
+  for (int cv = RING ? min(at.tx, nvec - 1) : at.tx; cv < nvec; cv += RING ? nvec : at.TX) {
     F2 nmean[S::NR], rstd[S::NR], m1[S::NR], m2[S::NR], w[S::NP], b[S::NP];
     S::load(stats, 2, cv * V, p.cg, nmean);
 #pragma unroll
@@ -581,25 +665,29 @@ __global__ void __launch_bounds__(kGnThreads, 2)
     const T* px = x + ch.row0 * p.xs + cv * V;
     const T* pd = dy + ch.row0 * p.c + cv * V;
     T* po = dx + ch.row0 * p.c + cv * V;
-    Pack<T, V> v[2 * kGnBwdBatch], g[2 * kGnBwdBatch];
-    for_rows<kGnBwdBatch>(
-        ch.rows, at,
-        [&](int u, int r) {
-          v[u].load_last(px + static_cast<int64_t>(r) * p.xs);
-          g[u].load_last(pd + static_cast<int64_t>(r) * p.c);
-        },
-        [&](int u, int r) {
-          Pack<T, V> o;
+    auto put = [&](const Pack<T, V>& v, const Pack<T, V>& g, int r) {
+      Pack<T, V> o;
 #pragma unroll
-          for (int i = 0; i < S::NP; ++i) {
-            F2 xhat;
-            const int k = S::of(i);
-            const F2 dz = gn_dz(get_pair<T, V>(v[u], i), get_pair<T, V>(g[u], i), nmean[k], rstd[k], w[i], b[i], p.silu,
-                                xhat);
-            put_pair<T, V>(o, i, mul_f2(rstd[k], fma_f2(xhat, m2[k], fma_f2(w[i], dz, m1[k]))));
-          }
-          o.store(po + static_cast<int64_t>(r) * p.c);
-        });
+      for (int i = 0; i < S::NP; ++i) {
+        F2 xhat;
+        const int k = S::of(i);
+        const F2 dz = gn_dz(get_pair<T, V>(v, i), get_pair<T, V>(g, i), nmean[k], rstd[k], w[i], b[i], p.silu, xhat);
+        put_pair<T, V>(o, i, mul_f2(rstd[k], fma_f2(xhat, m2[k], fma_f2(w[i], dz, m1[k]))));
+      }
+      o.store(po + static_cast<int64_t>(r) * p.c);
+    };
+    if constexpr (RING) {
+      ring_rows<2, T, V>(p, ch, at, s_m2 + p.groups, p.x, p.dy, true, put);
+    } else {
+      Pack<T, V> v[2 * kGnBwdBatch], g[2 * kGnBwdBatch];
+      for_rows<kGnBwdBatch>(
+          ch.rows, at,
+          [&](int u, int r) {
+            v[u].load_last(px + static_cast<int64_t>(r) * p.xs);
+            g[u].load_last(pd + static_cast<int64_t>(r) * p.c);
+          },
+          [&](int u, int r) { put(v[u], g[u], r); });
+    }
   }
 }
 
@@ -680,6 +768,19 @@ cudaError_t launch_ex(Handle* h, void (*kernel)(P...), int grid, size_t smem, in
   return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
+// Whether the rows go through the ring of bulk copies: dense, in 16-byte
+// vectors, no row longer than half a block, and blocks enough per chunk.
+template <typename T, int V>
+bool gn_ring(const GnParams& p) {
+  const int nvec = p.c / V;
+  return V * sizeof(T) == 16 && p.xs == p.c && nvec <= kGnThreads && p.chunk >= 8 * (kGnThreads / nvec);
+}
+
+template <typename... P>
+cudaError_t gn_ring_smem(void (*kernel)(P...), size_t bytes) {
+  return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
+}
+
 // Sequences up to this many bytes per CTA of a cluster of eight take one kernel.
 constexpr int64_t kGnClusterBytes = 64 * 1024;
 constexpr int kGnClusterMax = 8;
@@ -714,9 +815,21 @@ sc_status gn_forward_v(Handle* h, GnParams p, const int32_t* cu, int batch) {
       dev_free(h, call.table);
       return cuda_error(h, e, "group norm workspace");
     }
+    const size_t sums = gn_sum_smem(p.c, p.c / V), norms = sizeof(float) * 2 * p.groups;
     ++h->launches;
-    k_gn_stats<T, V><<<p.items, kGnThreads, gn_sum_smem(p.c, p.c / V), h->stream>>>(p, call.plan);
-    e = launch_ex(h, k_gn_apply<T, V, GS>, p.items, sizeof(float) * 2 * p.groups, 0, p, call.plan);
+    if (gn_ring<T, V>(p)) {
+      if constexpr (V * sizeof(T) == 16) {
+        e = gn_ring_smem(k_gn_stats<T, V, true>, kGnRingSmem);
+        if (e == cudaSuccess) e = gn_ring_smem(k_gn_apply<T, V, GS, true>, kGnRingSmem + 2 * sizeof(float) * 4096);
+        if (e == cudaSuccess) {
+          k_gn_stats<T, V, true><<<p.items, kGnThreads, kGnRingSmem, h->stream>>>(p, call.plan);
+          e = launch_ex(h, k_gn_apply<T, V, GS, true>, p.items, kGnRingSmem + norms, 0, p, call.plan);
+        }
+      }
+    } else {
+      k_gn_stats<T, V, false><<<p.items, kGnThreads, sums, h->stream>>>(p, call.plan);
+      e = launch_ex(h, k_gn_apply<T, V, GS, false>, p.items, norms, 0, p, call.plan);
+    }
   }
   if (e == cudaSuccess) e = cudaGetLastError();
   dev_free(h, p.part);
@@ -742,10 +855,22 @@ sc_status gn_backward_v(Handle* h, GnParams p, const int32_t* cu, int batch) {
   p.chan = reinterpret_cast<float*>(ws + part);
   const int dx_items = p.dx ? p.items : 0;
   const int chan_ctas = p.dw || p.db ? (p.c + kGnChanBlock - 1) / kGnChanBlock : 0;
+  const size_t sums = gn_sum_smem(p.c, p.c / V), norms = sizeof(float) * 2 * std::max(p.groups, kGnThreads);
   ++h->launches;
-  k_gn_bwd_sums<T, V, GS><<<p.items, kGnThreads, gn_sum_smem(p.c, p.c / V), h->stream>>>(p, call.plan);
-  e = launch_ex(h, k_gn_bwd_apply<T, V, GS>, dx_items + chan_ctas, sizeof(float) * 2 * std::max(p.groups, kGnThreads), 0,
-                p, call.plan, chan_ctas);
+  if (gn_ring<T, V>(p)) {
+    if constexpr (V * sizeof(T) == 16) {
+      e = gn_ring_smem(k_gn_bwd_sums<T, V, GS, true>, kGnRingSmem);
+      if (e == cudaSuccess) e = gn_ring_smem(k_gn_bwd_apply<T, V, GS, true>, kGnRingSmem + 2 * sizeof(float) * 4096);
+      if (e == cudaSuccess) {
+        k_gn_bwd_sums<T, V, GS, true><<<p.items, kGnThreads, kGnRingSmem, h->stream>>>(p, call.plan);
+        e = launch_ex(h, k_gn_bwd_apply<T, V, GS, true>, dx_items + chan_ctas, kGnRingSmem + norms, 0, p, call.plan,
+                      chan_ctas);
+      }
+    }
+  } else {
+    k_gn_bwd_sums<T, V, GS, false><<<p.items, kGnThreads, sums, h->stream>>>(p, call.plan);
+    e = launch_ex(h, k_gn_bwd_apply<T, V, GS, false>, dx_items + chan_ctas, norms, 0, p, call.plan, chan_ctas);
+  }
   if (e == cudaSuccess) e = cudaGetLastError();
   dev_free(h, ws);
   dev_free(h, call.table);
@@ -785,7 +910,7 @@ sc_status group_norm(Handle* h, const void* x, int64_t x_stride, const void* wei
                      sc_dtype dtype, sc_dtype wdtype) {
   GnParams p{};
   p.x = x; p.xs = x_stride; p.w = weight; p.b = bias; p.wdtype = wdtype; p.y = y; p.stats = stats;
-  p.c = c; p.groups = groups; p.cg = c / groups; p.eps = eps; p.silu = silu;
+  p.c = c; p.groups = groups; p.cg = c / groups; p.eps = eps; p.silu = silu; p.err = h->derr;
   if (dtype == SC_F32) return gn_dispatch<float>(h, p, cu, batch, false);
   if (dtype == SC_BF16) return gn_dispatch<__nv_bfloat16>(h, p, cu, batch, false);
   return gn_dispatch<__half>(h, p, cu, batch, false);
@@ -798,7 +923,7 @@ sc_status group_norm_backward(Handle* h, const void* x, int64_t x_stride, const 
   GnParams p{};
   p.x = x; p.xs = x_stride; p.dy = dy; p.w = weight; p.b = bias; p.wdtype = wdtype;
   p.stats = const_cast<float*>(stats); p.dx = dx; p.dw = dweight; p.db = dbias;
-  p.c = c; p.groups = groups; p.cg = c / groups; p.silu = silu;
+  p.c = c; p.groups = groups; p.cg = c / groups; p.silu = silu; p.err = h->derr;
   if (dtype == SC_F32) return gn_dispatch<float>(h, p, cu, batch, true);
   if (dtype == SC_BF16) return gn_dispatch<__nv_bfloat16>(h, p, cu, batch, true);
   return gn_dispatch<__half>(h, p, cu, batch, true);
