@@ -15,7 +15,7 @@
 // dK / dV kernel instead would save the second recomputation, but needs sums
 // across CTAs whose order changes from run to run.
 //   warp 0     TMA producer: X's Q / K pair and its dO / V once, then Y's tiles
-//              (and, for keys, the rows' statistics) into a ring
+//              (and, for keys, the queries' statistics) into a ring
 //   warp 1     issues S_m = X_m Y_m^T and dP into tensor memory
 //   warp 3     issues the accumulations dX_m += dS_m Y_m, dV += P dO with dS and
 //              P as A operands in tensor memory, Y MN-major
@@ -26,6 +26,13 @@
 // beside the accumulators fill it), but a group takes its row of S, then of dP,
 // into registers at once, which frees them for the other group's step; so one
 // group's exponentials run beside the other's products.
+// Where X are keys, lse and delta belong to the columns.  Read from shared
+// memory they cost 48 16-byte loads per thread and step beside the products'
+// operands (565 of 1,274 us at 8,192 + 2,777 tokens and 8 heads), so the tensor
+// cores add them: each statistic is split into three values of the input type
+// (24 bits and more) and enters as one more K step of its product, against rows
+// of a constant: S_m - lse_m / c and dP - delta_1 come out of tensor memory, and
+// so does delta_1 - delta_2 for the 32 columns that still fit.
 // Few CTAs: the walk is cut into ranges whose f32 sums k_da_bwd_join adds in order.
 // Every mbarrier wait is bounded (SC_ETIMEOUT).
 #include "sc_diffattn_dev.cuh"
@@ -48,12 +55,18 @@ struct Cfg {
   static constexpr int kY = 48;                        // rows of Y per step
   static constexpr int kStages = 5;
   static constexpr int kYBytes = kY * kDaD * 2;
-  static constexpr int kStage = 4 * kYBytes + (KV ? 1024 : 0);  // Y_1, Y_2, halves of the 128-wide one, statistics
-  static constexpr int kOffBar = kOffY + kStages * kStage;
+  // Y_1, Y_2, halves of the 128-wide one; statistics: 16-byte rows for S_1, S_2
+  // and dP (kY each) and of delta_1 - delta_2 (kDiff), and the rest of it in f32
+  static constexpr int kDiff = 32, kStatBytes = 16 * kY, kDiffBytes = 16 * kDiff, kRestBytes = 4 * (kY - kDiff);
+  static constexpr int kStage = 4 * kYBytes + (KV ? 3072 : 0);
+  static_assert(3 * kStatBytes + kDiffBytes + kRestBytes <= 3072, "stage");
+  // constant rows against the statistics of S and of dP (128 of 16 bytes), and zeros
+  static constexpr int kOffOnes = kOffY + kStages * kStage, kOffZero = kOffOnes + 2 * kX * 16;
+  static constexpr int kOffBar = kOffZero + kX * 16;
   static constexpr int kSmem = kOffBar + 256 + 1024;
-  // tensor memory columns: S_1 S_2 dP [P] dS_1 dS_2, then the accumulators
-  static constexpr uint32_t kS = 0, kDp = 2 * kY, kP = 3 * kY, kDs = KV ? 3 * kY + kY / 2 : 3 * kY, kAcc = 256,
-                            kV = 384;
+  // tensor memory columns: S_1 S_2 dP [delta_1 - delta_2, P] dS_1 dS_2, then the accumulators
+  static constexpr uint32_t kS = 0, kDp = 2 * kY, kD = 3 * kY, kP = kD + kDiff, kDs = KV ? kP + kY / 2 : 3 * kY,
+                            kAcc = 256, kV = 384;
   static_assert(kDs + kY <= kAcc, "tensor memory");
 };
 
@@ -62,8 +75,9 @@ struct DaBwd {
   const float* lse;    // [2][heads][nq]
   const float* maps;   // [nq][heads][2][128]
   const void* dout;
-  float* st;           // [4][heads][np]: -lse_1, -lse_2, -delta_1, -delta_2
-  int64_t np;          // rows of st: sequences start at multiples of 4
+  float* st;           // [5][heads][np]: -lse_1, -lse_2, -delta_1, -delta_2, delta_1 - delta_2
+  uint4* split;        // [4][heads][np] rows of eight values: -lse_m / c, -delta_1, delta_1 - delta_2 in three parts
+  int64_t np;          // rows of st and split: sequences start at multiples of 4
   void *dq, *dk, *dv, *dlam;
   float* part;         // [splits][rows of X][heads of X][dX_1 dX_2 (dV)], when the walk is cut
   int64_t nx;          // rows of X in all
@@ -83,6 +97,16 @@ __device__ __forceinline__ unsigned long long mul_f2(unsigned long long a, unsig
   asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
   return d;
 }
+// The constants that the split statistics are multiplied by.  bf16 has f32's
+// range.  f16: lse / c up to 65,504 * 256 with steps of 2^-16 (a score's unit:
+// 3e-6 of a weight at the usual scale), delta up to 65,504 * 16 with steps of 2^-20.
+template <typename T> struct SplitRange {
+  static constexpr float kS = 1.f, kDelta = 1.f, kMost = 1e30f;
+};
+template <> struct SplitRange<__half> {
+  static constexpr float kS = 256.f, kDelta = 16.f, kMost = 65504.f;
+};
+
 // Statistics of every (row, head), one warp each.  Records: aux = the
 // sequence's first row in st.
 template <typename T>
@@ -99,12 +123,22 @@ __global__ void __launch_bounds__(256) k_da_stats(const DaBwd p, const __grid_co
   const float g0 = Cvt<T>::to_f(g[0]), g1 = Cvt<T>::to_f(g[1]), g2 = Cvt<T>::to_f(g[2]), g3 = Cvt<T>::to_f(g[3]);
   const float d1 = warp_add(fmaf(g0, o1.x, g1 * o1.y) + fmaf(g2, o1.z, g3 * o1.w));
   const float d2 = warp_add(fmaf(g0, o2.x, g1 * o2.y) + fmaf(g2, o2.z, g3 * o2.w));
-  if (lane < 4) {
-    const float v = lane < 2 ? p.lse[(static_cast<int64_t>(lane) * p.heads + h) * p.nq + row] : lane == 2 ? d1 : d2;
-    float* dst = p.st + (static_cast<int64_t>(lane) * p.heads + h) * p.np + r.aux + (row - r.q0);
-    dst[0] = -v;
+  if (lane < 5) {
+    const float l = lane < 2 ? p.lse[(static_cast<int64_t>(lane) * p.heads + h) * p.nq + row] : 0.f;
+    const float v = lane < 2 ? -l : lane == 2 ? -d1 : lane == 3 ? -d2 : d1 - d2;
+    const int64_t at_st = (static_cast<int64_t>(lane) * p.heads + h) * p.np + r.aux + (row - r.q0);
+    p.st[at_st] = v;
     if (row == r.q1 - 1)  // up to three rows between sequences
-      for (int i = 1; (r.aux + row - r.q0 + i) & 3; ++i) dst[i] = 0.f;
+      for (int i = 1; (r.aux + row - r.q0 + i) & 3; ++i) p.st[at_st + i] = 0.f;
+  }
+  if (lane < 4) {
+    const float l = lane < 2 ? p.lse[(static_cast<int64_t>(lane) * p.heads + h) * p.nq + row] : 0.f;
+    const float raw_v = lane < 2 ? -l / p.scale_log2 : lane == 2 ? -d1 : d1 - d2;
+    const float most = SplitRange<T>::kMost;
+    const float v = fminf(fmaxf(raw_v * (lane < 2 ? 1.f / SplitRange<T>::kS : 1.f / SplitRange<T>::kDelta), -most), most);
+    const float hi = Cvt<T>::to_f(Cvt<T>::from_f(v)), mid = Cvt<T>::to_f(Cvt<T>::from_f(v - hi));
+    p.split[(static_cast<int64_t>(lane) * p.heads + h) * p.np + r.aux + (row - r.q0)] =
+        make_uint4(pack2<T>(hi, mid), pack2<T>(v - hi - mid, 0.f), 0u, 0u);
   }
 }
 
@@ -197,6 +231,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     tmem_alloc(smem_u32(s_tmem), kTmem);
     tmem_relinquish();
   }
+  if (KV) {
+    uint4* ones = reinterpret_cast<uint4*>(smem + C::kOffOnes);
+    for (int i = threadIdx.x; i < 3 * kX; i += kThreads) {
+      const float one = i < kX ? SplitRange<T>::kS : SplitRange<T>::kDelta;
+      ones[i] = i < 2 * kX ? make_uint4(pack2<T>(one, one), pack2<T>(one, 0.f), 0u, 0u) : make_uint4(0u, 0u, 0u, 0u);
+    }
+    fence_proxy_async_smem();
+  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -218,15 +260,18 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (!mbar_wait(y_empty0 + 8 * st, (use & 1) ^ 1, p.err)) break;
           const uint32_t yb = sbase + kOffY + st * C::kStage, bar = y_full0 + 8 * st;
           const int yr = y0 + ty * kY, yrow = (KV ? rec.q0 : rec.k0) + yr;
-          mbar_arrive_expect_tx(bar, 4 * kYBytes + (KV ? 4 * kY * 4 : 0));
+          mbar_arrive_expect_tx(bar, 4 * kYBytes + (KV ? 3 * C::kStatBytes + C::kDiffBytes + C::kRestBytes : 0));
           tma_load_3d(yb, &tmY, 0, 2 * yh, yrow, bar);
           tma_load_3d(yb + kYBytes, &tmY, 0, 2 * yh + 1, yrow, bar);
           tma_load_3d(yb + 2 * kYBytes, &tmYw, 0, yh, yrow, bar);
           tma_load_3d(yb + 3 * kYBytes, &tmYw, 64, yh, yrow, bar);
-          if (KV)  // st rows start at multiples of 4: 16-byte aligned; st goes on behind its last row
-            for (int k = 0; k < 4; ++k)
-              bulk_load(yb + 4 * kYBytes + k * kY * 4,
-                        p.st + (static_cast<int64_t>(k) * p.heads + yh) * p.np + rec.aux + yr, kY * 4, bar);
+          if (KV) {  // st rows start at multiples of 4: 16-byte aligned; both go on behind their last row
+            const int64_t at = static_cast<int64_t>(yh) * p.np + rec.aux + yr, step = static_cast<int64_t>(p.heads) * p.np;
+            const uint32_t sb = yb + 4 * kYBytes;
+            for (int k = 0; k < 3; ++k) bulk_load(sb + k * C::kStatBytes, p.split + k * step + at, C::kStatBytes, bar);
+            bulk_load(sb + 3 * C::kStatBytes, p.split + 3 * step + at, C::kDiffBytes, bar);
+            bulk_load(sb + 3 * C::kStatBytes + C::kDiffBytes, p.st + 4 * step + at + C::kDiff, C::kRestBytes, bar);
+          }
           if (++ty == ny) ty = 0, yh += KV ? 1 : 0;
           if (++st == kStages) st = 0, ++use;
         }
@@ -237,6 +282,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint32_t id_s = idesc_f16(128, kY, std::is_same_v<T, __nv_bfloat16>);
         const uint64_t x1 = smem_desc(sbase + kOffX, 1024, 2), xw = x1 + 2 * kXBytes / 16;
         const uint64_t y1d = smem_desc(sbase + kOffY, 1024, 2);
+        const uint32_t id_d = idesc_f16(128, C::kDiff, std::is_same_v<T, __nv_bfloat16>);
+        // constant rows, and a tile's statistics; the second half of their K step is zeros
+        const uint64_t one_s = smem_desc_plain(sbase + C::kOffOnes, C::kOffZero - C::kOffOnes, 128);
+        const uint64_t one_d = smem_desc_plain(sbase + C::kOffOnes + kX * 16, kX * 16, 128);
+        auto stat_desc = [&](uint32_t a) { return smem_desc_plain(a, sbase + C::kOffZero - a, 128); };
+        auto place = [&](uint64_t yd) { return static_cast<uint32_t>(yd - y1d) * 16u; };  // of a tile in the ring
         int ty = t0 % ny, st = 0, use = 0, asked = 0;  // tile and ring place of the next step to land; tiles to zero
         auto land = [&]() {
           bool r = mbar_wait(y_full0 + 8 * st, use & 1, p.err);
@@ -256,6 +307,12 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int k = 0; k < kDaD / 16; ++k)  // 32 bytes a step, in units of 16
               tc_mma_f16(tmem + C::kS + kY * m, x1 + m * (kXBytes / 16) + 2 * k, yd + m * (kYBytes / 16) + 2 * k, id_s,
                          k > 0 ? 1u : 0u);
+          if (KV) {
+            const uint32_t sb = sbase + kOffY + place(yd) + 4 * kYBytes;
+#pragma unroll
+            for (int m = 0; m < 2; ++m)
+              tc_mma_f16(tmem + C::kS + kY * m, one_s, stat_desc(sb + m * C::kStatBytes), id_s, 1u);
+          }
           tc_commit(s_full0 + 8u * (j & 1));
         };
         auto issue_dp = [&](int j, uint64_t yd) {
@@ -263,6 +320,11 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int k = 0; k < kDaDv / 16; ++k)
             tc_mma_f16(tmem + C::kDp, xw + (k / 4) * (kXBytes / 16) + 2 * (k % 4),
                        yd + (2 + k / 4) * (kYBytes / 16) + 2 * (k % 4), id_s, k > 0 ? 1u : 0u);
+          if (KV) {
+            const uint32_t sb = sbase + kOffY + place(yd) + 4 * kYBytes;
+            tc_mma_f16(tmem + C::kDp, one_d, stat_desc(sb + 2 * C::kStatBytes), id_s, 1u);
+            tc_mma_f16(tmem + C::kD, one_d, stat_desc(sb + 3 * C::kStatBytes), id_d, 0u);
+          }
           tc_commit(dp_full0 + 8u * (j & 1));
         };
         bool ok = mbar_wait(x_full, 0, p.err) && land();
@@ -382,7 +444,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int c0 = y0 + ty * kY;
       const uint32_t turn = (j >> 1) & 1;
       const bool full = c0 >= lo_max && c0 + kY <= hi_min;
-      const float4* st = reinterpret_cast<const float4*>(smem + kOffY + place * C::kStage + 4 * kYBytes);
+      const float4* rest = reinterpret_cast<const float4*>(smem + kOffY + place * C::kStage + 4 * kYBytes +
+                                                           3 * C::kStatBytes + C::kDiffBytes);
       ok = warp_wait(s_full0 + 8u * grp, turn, p.err);
       // the statistics landed with the tile: the MMA thread has seen that, this one has not
       if (KV) ok = ok && warp_wait(y_full0 + 8 * place, use, p.err);
@@ -395,16 +458,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (lane == 0) mbar_arrive(s_free);
       auto weights = [&](int m) {
 #pragma unroll
-        for (int i = 0; i < kY; i += 4) {
-          float4 l4 = make_float4(nl[m], nl[m], nl[m], nl[m]);
-          if (KV) l4 = st[kY / 4 * m + i / 4];
+        for (int i = 0; i < kY; i += 2) {
+          const unsigned long long x2 = f2(w[m][i], w[m][i + 1]);
           float a, b;
-          f2_split(fma_f2(f2(w[m][i], w[m][i + 1]), sc2, f2(l4.x, l4.y)), a, b);
+          f2_split(KV ? mul_f2(x2, sc2) : fma_f2(x2, sc2, f2(nl[m], nl[m])), a, b);
           w[m][i] = ex2_ftz(a);
           w[m][i + 1] = ex2_ftz(b);
-          f2_split(fma_f2(f2(w[m][i + 2], w[m][i + 3]), sc2, f2(l4.z, l4.w)), a, b);
-          w[m][i + 2] = ex2_ftz(a);
-          w[m][i + 3] = ex2_ftz(b);
         }
       };
       weights(0);
@@ -412,6 +471,19 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (!ok) break;
       tc_fence_after();
       tmem_ld48(lane_base + C::kDp, dp);
+      float diff[kY];  // delta_1 - delta_2 (of the columns; where X are queries, of the row)
+      if constexpr (KV) {
+        float d[C::kDiff];
+        tmem_ld32(lane_base + C::kD, d);
+#pragma unroll
+        for (int i = 0; i < kY; i += 4) {
+          const float4 r4 = i < C::kDiff ? make_float4(d[i], d[i + 1], d[i + 2], d[i + 3]) : rest[(i - C::kDiff) / 4];
+          diff[i] = r4.x;
+          diff[i + 1] = r4.y;
+          diff[i + 2] = r4.z;
+          diff[i + 3] = r4.w;
+        }
+      }
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(dp_free);
@@ -425,45 +497,31 @@ __global__ void __launch_bounds__(kThreads, 1)
           w[0][i] = see ? w[0][i] : 0.f;
           w[1][i] = see ? w[1][i] : 0.f;
           dp[i] = see ? dp[i] : 0.f;
+          if (KV) diff[i] = see ? diff[i] : 0.f;
         }
       }
       const unsigned long long nlam2 = f2(nlam, nlam);
       uint32_t pk[kY / 16][8], k1[kY / 16][8], k2[kY / 16][8];
 #pragma unroll
-      for (int c = 0; c < kY; c += 16) {
-#pragma unroll
-        for (int i = 0; i < 16; i += 4) {
-          float4 d1 = make_float4(nd[0], nd[0], nd[0], nd[0]), d2 = make_float4(nd[1], nd[1], nd[1], nd[1]);
-          if (KV) {
-            d1 = st[kY / 2 + (c + i) / 4];
-            d2 = st[3 * kY / 4 + (c + i) / 4];
-            if (!full) {
-              float* e1 = &d1.x;
-              float* e2 = &d2.x;
-#pragma unroll
-              for (int k = 0; k < 4; ++k) {
-                const bool see = c0 + c + i + k >= lo && c0 + c + i + k < hi;
-                e1[k] = see ? e1[k] : 0.f;
-                e2[k] = see ? e2[k] : 0.f;
-              }
-            }
-          }
-#pragma unroll
-          for (int k = 0; k < 4; k += 2) {
-            const int e = c + i + k;
-            const unsigned long long dd = f2(dp[e], dp[e + 1]);
-            const unsigned long long w1 = f2(w[0][e], w[0][e + 1]);
-            const unsigned long long w2 = mul_f2(nlam2, f2(w[1][e], w[1][e + 1]));  // -lam P_2
-            float a, b;
-            f2_split(mul_f2(w1, add_f2(dd, k ? f2(d1.z, d1.w) : f2(d1.x, d1.y))), a, b);
-            k1[c / 16][(i + k) / 2] = pack2<T>(a, b);
-            f2_split(mul_f2(w2, add_f2(dd, k ? f2(d2.z, d2.w) : f2(d2.x, d2.y))), a, b);
-            k2[c / 16][(i + k) / 2] = pack2<T>(a, b);
-            if (KV) {
-              f2_split(add_f2(w1, w2), a, b);
-              pk[c / 16][(i + k) / 2] = pack2<T>(a, b);
-            }
-          }
+      for (int e = 0; e < kY; e += 2) {
+        // dP - delta_1 and dP - delta_2
+        unsigned long long d1 = f2(dp[e], dp[e + 1]), d2;
+        if (KV) {
+          d2 = add_f2(d1, f2(diff[e], diff[e + 1]));
+        } else {
+          d2 = add_f2(d1, f2(nd[1], nd[1]));
+          d1 = add_f2(d1, f2(nd[0], nd[0]));
+        }
+        const unsigned long long w1 = f2(w[0][e], w[0][e + 1]);
+        const unsigned long long w2 = mul_f2(nlam2, f2(w[1][e], w[1][e + 1]));  // -lam P_2
+        float a, b;
+        f2_split(mul_f2(w1, d1), a, b);
+        k1[e / 16][e % 16 / 2] = pack2<T>(a, b);
+        f2_split(mul_f2(w2, d2), a, b);
+        k2[e / 16][e % 16 / 2] = pack2<T>(a, b);
+        if (KV) {
+          f2_split(add_f2(w1, w2), a, b);
+          pk[e / 16][e % 16 / 2] = pack2<T>(a, b);
         }
       }
       // the columns of the step before are read: only these stores and the
@@ -654,8 +712,10 @@ sc_status run_backward(Handle* h, const DaArgs& a) {
     if (rows > 0x7fffff00) return set_error(h, SC_EINVAL, "differential attention backward: too many rows");
   }
   p.np = rows + Cfg<true>::kY;  // a tile's copy may reach behind the last row
-  cudaError_t e = dev_alloc(h, reinterpret_cast<void**>(&p.st), sizeof(float) * 4 * a.heads * p.np);
+  const size_t per = static_cast<size_t>(a.heads) * p.np;
+  cudaError_t e = dev_alloc(h, reinterpret_cast<void**>(&p.split), per * (4 * sizeof(uint4) + 5 * sizeof(float)));
   if (e != cudaSuccess) return cuda_error(h, e, "differential attention workspace");
+  p.st = reinterpret_cast<float*>(p.split + 4 * per);
   sc_status st = SC_OK;
   if (nq > 0) {
     SeqPlan plan;
@@ -674,7 +734,7 @@ sc_status run_backward(Handle* h, const DaArgs& a) {
   if (st == SC_OK && (a.dk || a.dv)) st = launch_bwd<T, true>(h, a, p, st_row);
   if (st == SC_OK && a.dq) st = launch_bwd<T, false>(h, a, p, st_row);
   e = cudaGetLastError();
-  dev_free(h, p.st);
+  dev_free(h, p.split);
   if (st != SC_OK) return st;
   return e == cudaSuccess ? SC_OK : cuda_error(h, e, "differential attention backward launch");
 }

@@ -185,6 +185,12 @@ __device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&v)[8])
                : "memory");
 }
 
+// Descriptor of a K-major operand without swizzle: 8-row groups of 16-byte rows
+// `sbo` bytes apart, the two halves of a 16-wide K step `lbo` bytes apart.
+__device__ __forceinline__ uint64_t smem_desc_plain(uint32_t addr, uint32_t lbo, uint32_t sbo) {
+  return (smem_desc(addr, sbo, 0) & ~(0x3FFFull << 16)) | (static_cast<uint64_t>((lbo >> 4) & 0x3FFFu) << 16);
+}
+
 // Register split of a 384-thread block launched with 168 registers a thread:
 // warps 0-3 keep 72, warps 4-11 take 216 (128 * 72 + 256 * 216 = 384 * 168).
 __device__ __forceinline__ void regs_release() { asm volatile("setmaxnreg.dec.sync.aligned.u32 72;"); }
