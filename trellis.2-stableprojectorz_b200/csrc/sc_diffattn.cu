@@ -251,8 +251,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(s_free);
-        // asked for here, looked at behind the maximum
-        const bool o_ready = j == 0 || mbar_try_wait(o_done0 + 8u * m, (j - 1) & 1);
         if (!full) {
 #pragma unroll
           for (int i = 0; i < kTile; ++i) s[i / 64][i % 64] = i < valid ? s[i / 64][i % 64] : -INFINITY;  // 2^-inf = 0
@@ -269,7 +267,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const float alpha = move ? ex2_ftz(mx - m_new) : 1.f;
         // the product of this map's last step: O_m is complete and P_m is read
         if (j > 0) {
-          if (!__all_sync(0xffffffffu, o_ready) && !warp_wait(o_done0 + 8u * m, (j - 1) & 1, p.err)) {
+          if (!warp_wait(o_done0 + 8u * m, (j - 1) & 1, p.err)) {
             ok = false;
             break;
           }

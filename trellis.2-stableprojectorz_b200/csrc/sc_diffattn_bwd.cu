@@ -487,8 +487,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(dp_free);
-      // asked for here, looked at when the results are ready to be stored
-      const bool p_ready = j == 0 || mbar_try_wait(p_free0 + 8u * (grp ^ 1), ((j - 1) >> 1) & 1);
       weights(1);
       if (!full) {  // weight 0, and 0 * NaN of a row that is not seen
 #pragma unroll
@@ -525,8 +523,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
       // the columns of the step before are read: only these stores and the
-      // products stand between one step's wait here and the next one's
-      if (!__all_sync(0xffffffffu, p_ready)) ok = warp_wait(p_free0 + 8u * (grp ^ 1), ((j - 1) >> 1) & 1, p.err);
+      // products stand between one step's wait here and the next one's.  (A try
+      // ahead of need would suspend the warp: 902 against 757 us for dk and dv.)
+      if (j > 0) ok = warp_wait(p_free0 + 8u * (grp ^ 1), ((j - 1) >> 1) & 1, p.err);
       if (!ok) break;
       tc_fence_after();
 #pragma unroll
