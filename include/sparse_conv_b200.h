@@ -324,7 +324,7 @@ typedef struct sc_diff_attention_args {
   int32_t batch, heads, kv_heads;
   int32_t lam_count;
   float lam_value;
-  float scale;              /* > 0, usually 1 / 8 */
+  float scale;              /* 2^-20 .. 2^20, usually 1 / 8 */
   int32_t causal;
   sc_dtype dtype, lam_dtype;
   /* forward: out is written; lse [2][heads][Nq] (log-sum-exp in base 2) and

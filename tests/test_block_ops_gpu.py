@@ -67,7 +67,8 @@ def _gn_check(pkg, cuda, lens, c, groups, dtype, wdtype, silu, seed=0, eps=1e-5)
 @pytest.mark.parametrize("dtype,wdtype", [(FP, FP), (BF, BF), (BF, FP), (HF, HF), (HF, FP)])
 @pytest.mark.parametrize("lens,c,groups", [
     ([300], 64, 32), ([1], 32, 8), ([2, 1, 0, 700, 33], 64, 4), ([129, 257], 36, 9), ([40, 3], 7, 7), ([65], 6, 1),
-    ([1000, 1500], 256, 32), ([17, 90], 4096, 32), ([50], 4095, 5), ([9001], 96, 3)])
+    ([1000, 1500], 256, 32), ([17, 90], 4096, 32), ([50], 4095, 5), ([9001], 96, 3), ([30], 4096, 4096),
+    ([700], 1024, 1024)])
 def test_group_norm(pkg, cuda, dtype, wdtype, lens, c, groups):
     _gn_check(pkg, cuda, lens, c, groups, dtype, wdtype, silu=True)
 
@@ -192,9 +193,10 @@ def _close(got, ref, name, u):
         assert _rel(g, r) < 2 * u + 2e-4, (name, _rel(g, r))
 
 
-def _da_check(pkg, cuda, lq, lk, heads, kv_heads, dtype, causal, seed=0, train=True, scale=None, spread=1.5):
+def _da_check(pkg, cuda, lq, lk, heads, kv_heads, dtype, causal, seed=0, train=True, scale=None, spread=1.5, gain=1.0):
     cq, ck = _cu(lq), _cu(lk)
     q, k, v, lam, dout = _da_inputs(cuda, cq[-1], ck[-1], heads, kv_heads, dtype, seed, spread)
+    dout = dout * gain
     with torch.no_grad():
         out = pkg.sparse_diff_attention(q, k, v, lam, cq, ck, scale, causal)
     u = _half(dtype)
@@ -253,6 +255,28 @@ def test_diff_attention_large_scores(pkg, cuda):
     """Scores of deviation 20: the softmax picks single keys, and the running maximum moves."""
     _da_check(pkg, cuda, [260, 30], [900, 300], 4, 2, BF, False, seed=23, spread=20.0, train=False)
     _da_check(pkg, cuda, [200], [200], 2, 2, HF, True, seed=24, scale=0.3, train=False)
+
+
+def test_diff_attention_scales_and_gains(pkg, cuda):
+    """The ends of the scale's range (at 2^-20 every weight is 1 / n), and gradients as a loss scale makes them."""
+    for dtype in (BF, HF):
+        _da_check(pkg, cuda, [150, 40], [150, 90], 2, 1, dtype, True, seed=32, scale=2.0 ** -20, train=False)
+        _da_check(pkg, cuda, [150, 40], [150, 90], 2, 1, dtype, False, seed=33, scale=2.0, spread=0.1)
+        _da_check(pkg, cuda, [150, 40], [150, 90], 2, 1, dtype, True, seed=34, gain=64.0)
+        _da_check(pkg, cuda, [150, 40], [150, 90], 2, 1, dtype, True, seed=35, gain=2.0 ** -6)
+    cu = [0, 100]
+    q, k, v, lam, dout = _da_inputs(cuda, 100, 100, 2, 2, HF, 36)
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+    got = torch.autograd.grad(pkg.sparse_diff_attention(q, k, v, lam, cu, scale=2.0 ** -20), leaves, dout)
+    ref = B.diff_attention(_f64(q), _f64(k), _f64(v), _f64(lam), cu, scale=2.0 ** -20, dout=_f64(dout), u=_half(HF))
+    _close(got[2], ref, "dv", _half(HF))
+
+
+def test_diff_attention_prefill_beside_single_tokens(pkg, cuda):
+    """Sequences whose keys are cut into ranges beside some whose are not."""
+    for dtype in (BF, HF):
+        _da_check(pkg, cuda, [1, 300, 2, 40], [5000, 300, 9000, 100], 4, 2, dtype, True, seed=37, train=False)
+    _da_check(pkg, cuda, [1, 200, 2], [2500, 200, 1200], 2, 1, BF, True, seed=38)
 
 
 def test_diff_attention_many_sequences(pkg, cuda):

@@ -249,7 +249,7 @@ def sparse_diff_attention(q, k, v, lam, cu_seqlens_q, cu_seqlens_kv=None, scale=
                     - lam_h softmax_j(scale q[i, 2h+1] . k[j, 2g+1]) v[j, g]
 
     ``cu_seqlens_q`` / ``cu_seqlens_kv`` as in ``sparse_attention`` (the latter
-    defaults to the former); ``scale`` defaults to ``1 / sqrt(64)``.  With
+    defaults to the former); ``scale`` (2^-20 to 2^20) defaults to ``1 / sqrt(64)``.  With
     ``causal`` query i of a sequence sees the keys ``j <= i + len_kv - len_q``
     (a single new token sees the whole cache).  Rows that see no key are zero.
     Returns ``(total_N, H, 128)``.
@@ -285,8 +285,8 @@ def sparse_diff_attention(q, k, v, lam, cu_seqlens_q, cu_seqlens_kv=None, scale=
     if len(cu_q) != len(cu_kv):
         raise ValueError("cu_seqlens_q and cu_seqlens_kv must have the same count")
     scale = 0.125 if scale is None else float(scale)
-    if not (scale > 0 and math.isfinite(scale)):
-        raise ValueError("scale must be positive and finite")
+    if not 2.0 ** -20 <= scale <= 2.0 ** 20:
+        raise ValueError("scale must lie in [2^-20, 2^20]")
     if not q.is_cuda:
         raise ValueError("sparse_diff_attention runs on CUDA tensors only")
     leaves = [t for t in (q, k, v, lam) if isinstance(t, torch.Tensor)]

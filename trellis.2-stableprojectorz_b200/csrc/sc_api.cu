@@ -612,7 +612,7 @@ sc_status da_args(Handle* H, const sc_diff_attention_args* a, bool backward, sc:
     return bad("need 1 <= heads <= 32767, a multiple of kv_heads");
   if (!offsets_ok(a->cu_seqlens_q, a->batch) || !offsets_ok(a->cu_seqlens_kv, a->batch))
     return bad("cu_seqlens must start at 0 and be non-decreasing");
-  if (!(a->scale > 0.f) || !(a->scale <= 3.0e38f)) return bad("scale must be positive and finite");
+  if (!(a->scale >= 0x1p-20f) || !(a->scale <= 0x1p20f)) return bad("scale must lie in [2^-20, 2^20]");
   if (a->lam) {
     if (a->lam_count != 1 && a->lam_count != a->heads) return bad("lam_count must be 1 or heads");
     if (a->lam_dtype != a->dtype && a->lam_dtype != SC_F32) return bad("lam must be in the dtype of q or f32");

@@ -57,8 +57,8 @@ struct DaFwd {
   void* out;
   float* lse;
   float* maps;
-  float* part_o;    // [splits][nq][heads][2][128], unnormalised
-  float4* part_ml;  // [splits][nq][heads] (max_1, sum_1, max_2, sum_2)
+  float* part_o;    // [part rows][heads][2][128], unnormalised: row part0 + range * rows + row of a cut sequence
+  float4* part_ml;  // [part rows][heads] (max_1, sum_1, max_2, sum_2)
   int64_t nq;
   int heads, rep, pack, tokens;  // rep = heads / kv_heads; heads and tokens of a tile (pack * tokens rows)
   int causal;
@@ -326,10 +326,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int64_t qrow = static_cast<int64_t>(rec.q0) + tok;
       const int64_t at = live ? qrow * p.heads + head : 0;
       const bool join = tile.nsplit > 1;
+      const int64_t part = (rec.part0 + static_cast<int64_t>(tile.split) * (rec.q1 - rec.q0) + tok) * p.heads + head;
       const float i1 = r1.y > 0.f ? 1.f / r1.y : 0.f, i2 = r2.y > 0.f ? 1.f / r2.y : 0.f;
       const float lam = live ? p.lam.get(head) : 0.f;
       if (live && join && m == 0)
-        p.part_ml[static_cast<int64_t>(tile.split) * p.nq * p.heads + at] = make_float4(r1.x, r1.y, r2.x, r2.y);
+        p.part_ml[part] = make_float4(r1.x, r1.y, r2.x, r2.y);
       if (live && !join && p.lse) {
         const float2 r = m ? r2 : r1;
         p.lse[(static_cast<int64_t>(m) * p.heads + head) * p.nq + qrow] = r.y > 0.f ? r.x + log2f(r.y) : INFINITY;
@@ -349,9 +350,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           o1[i] = r1.y > 0.f ? o1[i] * (join ? 1.f : i1) : 0.f;
           o2[i] = r2.y > 0.f ? o2[i] * (join ? 1.f : i2) : 0.f;
         }
-        float* f32 = join ? p.part_o + static_cast<int64_t>(tile.split) * p.nq * p.heads * (2 * kDaDv) : p.maps;
+        float* f32 = join ? p.part_o + part * (2 * kDaDv) : p.maps ? p.maps + at * (2 * kDaDv) : nullptr;
         if (live && f32) {
-          float4* dst = reinterpret_cast<float4*>(f32 + at * (2 * kDaDv) + d);
+          float4* dst = reinterpret_cast<float4*>(f32 + d);
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
             dst[i] = make_float4(o1[4 * i], o1[4 * i + 1], o1[4 * i + 2], o1[4 * i + 3]);
@@ -403,11 +404,12 @@ __global__ void __launch_bounds__(128) k_da_join(const DaFwd p, const __grid_con
   const SeqRec& r = plan.at(rec);
   const int nsplit = max(1, (r.k1 - r.k0 + p.split_keys - 1) / p.split_keys);
   if (nsplit == 1) return;
-  const int64_t step = p.nq * p.heads;
+  const int64_t step = static_cast<int64_t>(r.q1 - r.q0) * p.heads;
+  const int64_t part = (r.part0 + static_cast<int64_t>(row - r.q0)) * p.heads + h;
   float m1 = -INFINITY, m2 = -INFINITY, l1 = 0.f, l2 = 0.f, o1[4] = {}, o2[4] = {};
   for (int s0 = 0; s0 < nsplit; s0 += 32) {  // lane = range
     const int ns = min(32, nsplit - s0);
-    const float4 ml = lane < ns ? p.part_ml[(s0 + lane) * step + at] : make_float4(-INFINITY, 0.f, -INFINITY, 0.f);
+    const float4 ml = lane < ns ? p.part_ml[(s0 + lane) * step + part] : make_float4(-INFINITY, 0.f, -INFINITY, 0.f);
     float t1 = ml.x, t2 = ml.z;
 #pragma unroll
     for (int x = 16; x > 0; x >>= 1) {
@@ -434,7 +436,7 @@ __global__ void __launch_bounds__(128) k_da_join(const DaFwd p, const __grid_con
     }
 #pragma unroll 4
     for (int s = 0; s < ns; ++s) {
-      const float* o = p.part_o + ((s0 + s) * step + at) * (2 * kDaDv) + 4 * lane;
+      const float* o = p.part_o + ((s0 + s) * step + part) * (2 * kDaDv) + 4 * lane;
       const float4 a = *reinterpret_cast<const float4*>(o), b = *reinterpret_cast<const float4*>(o + kDaDv);
       const float u1 = __shfl_sync(0xffffffffu, w1, s), u2 = __shfl_sync(0xffffffffu, w2, s);
       const float av[4] = {a.x, a.y, a.z, a.w}, bv[4] = {b.x, b.y, b.z, b.w};
@@ -485,7 +487,8 @@ sc_status run_forward(Handle* h, const DaArgs& a) {
   p.err = h->derr;
   const int groups = a.heads / p.pack;
   // Work in key tiles; keys are cut into ranges only where whole tiles of rows
-  // would leave SMs without a CTA.
+  // would leave SMs without a CTA.  About two ranges per SM: at 24 single tokens
+  // against 513 to 16,084 keys 1 / 2 / 3 / 4 / 8 took 109 / 100 / 103 / 110 / 128 us.
   std::vector<SeqRec> recs;
   int64_t tiles = 0, work = 0;
   int32_t longest = 0;
@@ -500,21 +503,22 @@ sc_status run_forward(Handle* h, const DaArgs& a) {
   }
   p.split_keys = std::max(kTile, (longest + kTile - 1) / kTile * kTile);
   if (tiles < 2 * h->num_sms) {
-    const int64_t want = (work + 4ll * h->num_sms - 1) / (4ll * h->num_sms);
+    const int64_t want = (work + 2ll * h->num_sms - 1) / (2ll * h->num_sms);
     // four tiles at least: a shorter range costs less than the join
     p.split_keys = static_cast<int>(std::min<int64_t>(p.split_keys, std::max<int64_t>(4, want) * kTile));
   }
   // the longest first: the tail of the launch is made of short CTAs
   std::stable_sort(recs.begin(), recs.end(),
                    [](const SeqRec& x, const SeqRec& y) { return x.k1 - x.k0 > y.k1 - y.k0; });
-  int64_t items = 0, splits = 1;
+  int64_t items = 0, parts = 0;
   for (SeqRec& r : recs) {
     const int64_t s = std::max(1, (r.k1 - r.k0 + p.split_keys - 1) / p.split_keys);
     r.item0 = static_cast<int32_t>(items);
+    r.part0 = static_cast<int32_t>(parts);
     items += r.aux * s;
-    splits = std::max(splits, s);
+    if (s > 1) parts += s * (r.q1 - r.q0);
   }
-  if (items > 0x7fffffff || groups > 65535) return set_error(h, SC_EINVAL, "differential attention: too many tiles");
+  if (items > 0x7fffffff || parts > 0x7fffffff || groups > 65535) return set_error(h, SC_EINVAL, "differential attention: too many tiles");
   // q as [64][2 maps][heads][tokens], k as [64][2 kv heads][tokens], v as [128][kv heads][tokens]
   CUtensorMap tq, tk, tv;
   const uint64_t one = 1;
@@ -537,8 +541,8 @@ sc_status run_forward(Handle* h, const DaArgs& a) {
   if (st != SC_OK) return st;
   char* ws = nullptr;
   cudaError_t e = cudaSuccess;
-  if (splits > 1) {
-    const size_t n = static_cast<size_t>(splits) * nq * a.heads;
+  if (parts > 0) {
+    const size_t n = static_cast<size_t>(parts) * a.heads;
     e = dev_alloc(h, reinterpret_cast<void**>(&ws), n * (2 * kDaDv * sizeof(float) + sizeof(float4)));
     if (e != cudaSuccess) {
       dev_free(h, table);
@@ -551,7 +555,7 @@ sc_status run_forward(Handle* h, const DaArgs& a) {
   if (e == cudaSuccess) {
     ++h->launches;
     k_da_fwd<T><<<dim3(static_cast<unsigned>(items), groups), kThreads, kSmem, h->stream>>>(tq, tk, tv, p, plan);
-    if (splits > 1) {
+    if (parts > 0) {
       ++h->launches;
       k_da_join<T><<<static_cast<unsigned>((nq * a.heads + 3) / 4), 128, 0, h->stream>>>(
           p, plan, static_cast<int>(recs.size()));

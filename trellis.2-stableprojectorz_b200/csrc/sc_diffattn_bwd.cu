@@ -60,8 +60,8 @@ struct Cfg {
   static constexpr int kDiff = 32, kStatBytes = 16 * kY, kDiffBytes = 16 * kDiff, kRestBytes = 4 * (kY - kDiff);
   static constexpr int kStage = 4 * kYBytes + (KV ? 3072 : 0);
   static_assert(3 * kStatBytes + kDiffBytes + kRestBytes <= 3072, "stage");
-  // constant rows against the statistics of S and of dP (128 of 16 bytes), and zeros
-  static constexpr int kOffOnes = kOffY + kStages * kStage, kOffZero = kOffOnes + 2 * kX * 16;
+  // constant rows against the split statistics (128 of 16 bytes), and zeros
+  static constexpr int kOffOnes = kOffY + kStages * kStage, kOffZero = kOffOnes + kX * 16;
   static constexpr int kOffBar = kOffZero + kX * 16;
   static constexpr int kSmem = kOffBar + 256 + 1024;
   // tensor memory columns: S_1 S_2 dP [delta_1 - delta_2, P] dS_1 dS_2, then the accumulators
@@ -97,15 +97,21 @@ __device__ __forceinline__ unsigned long long mul_f2(unsigned long long a, unsig
   asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
   return d;
 }
-// The constants that the split statistics are multiplied by.  bf16 has f32's
-// range.  f16: lse / c up to 65,504 * 256 with steps of 2^-16 (a score's unit:
-// 3e-6 of a weight at the usual scale), delta up to 65,504 * 16 with steps of 2^-20.
-template <typename T> struct SplitRange {
-  static constexpr float kS = 1.f, kDelta = 1.f, kMost = 1e30f;
+// A statistic v as three values of T, v = k0 a + k1 b + k2 c.  bf16 has f32's
+// range.  f16: up to 65,504 * 1,024, in steps of 2^-34.
+template <typename T> struct Split {
+  static constexpr float k0 = 1.f, k1 = 1.f, k2 = 1.f, kMost = 1e38f;
 };
-template <> struct SplitRange<__half> {
-  static constexpr float kS = 256.f, kDelta = 16.f, kMost = 65504.f;
+template <> struct Split<__half> {
+  static constexpr float k0 = 1024.f, k1 = 1.f, k2 = 1.f / 1024.f, kMost = 65504.f * 1024.f;
 };
+template <typename T>
+__device__ __forceinline__ uint4 split3(float v) {
+  using S = Split<T>;
+  v = fminf(fmaxf(v, -S::kMost), S::kMost);
+  const float a = Cvt<T>::to_f(Cvt<T>::from_f(v / S::k0)), r = v - a * S::k0, b = Cvt<T>::to_f(Cvt<T>::from_f(r / S::k1));
+  return make_uint4(pack2<T>(a, b), pack2<T>((r - b * S::k1) / S::k2, 0.f), 0u, 0u);
+}
 
 // Statistics of every (row, head), one warp each.  Records: aux = the
 // sequence's first row in st.
@@ -133,12 +139,8 @@ __global__ void __launch_bounds__(256) k_da_stats(const DaBwd p, const __grid_co
   }
   if (lane < 4) {
     const float l = lane < 2 ? p.lse[(static_cast<int64_t>(lane) * p.heads + h) * p.nq + row] : 0.f;
-    const float raw_v = lane < 2 ? -l / p.scale_log2 : lane == 2 ? -d1 : d1 - d2;
-    const float most = SplitRange<T>::kMost;
-    const float v = fminf(fmaxf(raw_v * (lane < 2 ? 1.f / SplitRange<T>::kS : 1.f / SplitRange<T>::kDelta), -most), most);
-    const float hi = Cvt<T>::to_f(Cvt<T>::from_f(v)), mid = Cvt<T>::to_f(Cvt<T>::from_f(v - hi));
     p.split[(static_cast<int64_t>(lane) * p.heads + h) * p.np + r.aux + (row - r.q0)] =
-        make_uint4(pack2<T>(hi, mid), pack2<T>(v - hi - mid, 0.f), 0u, 0u);
+        split3<T>(lane < 2 ? -l / p.scale_log2 : lane == 2 ? -d1 : d1 - d2);
   }
 }
 
@@ -233,10 +235,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   if (KV) {
     uint4* ones = reinterpret_cast<uint4*>(smem + C::kOffOnes);
-    for (int i = threadIdx.x; i < 3 * kX; i += kThreads) {
-      const float one = i < kX ? SplitRange<T>::kS : SplitRange<T>::kDelta;
-      ones[i] = i < 2 * kX ? make_uint4(pack2<T>(one, one), pack2<T>(one, 0.f), 0u, 0u) : make_uint4(0u, 0u, 0u, 0u);
-    }
+    for (int i = threadIdx.x; i < 2 * kX; i += kThreads)
+      ones[i] = i < kX ? make_uint4(pack2<T>(Split<T>::k0, Split<T>::k1), pack2<T>(Split<T>::k2, 0.f), 0u, 0u)
+                       : make_uint4(0u, 0u, 0u, 0u);
     fence_proxy_async_smem();
   }
   tc_fence_before();
@@ -284,8 +285,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint64_t y1d = smem_desc(sbase + kOffY, 1024, 2);
         const uint32_t id_d = idesc_f16(128, C::kDiff, std::is_same_v<T, __nv_bfloat16>);
         // constant rows, and a tile's statistics; the second half of their K step is zeros
-        const uint64_t one_s = smem_desc_plain(sbase + C::kOffOnes, C::kOffZero - C::kOffOnes, 128);
-        const uint64_t one_d = smem_desc_plain(sbase + C::kOffOnes + kX * 16, kX * 16, 128);
+        const uint64_t one = smem_desc_plain(sbase + C::kOffOnes, C::kOffZero - C::kOffOnes, 128);
         auto stat_desc = [&](uint32_t a) { return smem_desc_plain(a, sbase + C::kOffZero - a, 128); };
         auto place = [&](uint64_t yd) { return static_cast<uint32_t>(yd - y1d) * 16u; };  // of a tile in the ring
         int ty = t0 % ny, st = 0, use = 0, asked = 0;  // tile and ring place of the next step to land; tiles to zero
@@ -311,7 +311,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             const uint32_t sb = sbase + kOffY + place(yd) + 4 * kYBytes;
 #pragma unroll
             for (int m = 0; m < 2; ++m)
-              tc_mma_f16(tmem + C::kS + kY * m, one_s, stat_desc(sb + m * C::kStatBytes), id_s, 1u);
+              tc_mma_f16(tmem + C::kS + kY * m, one, stat_desc(sb + m * C::kStatBytes), id_s, 1u);
           }
           tc_commit(s_full0 + 8u * (j & 1));
         };
@@ -322,8 +322,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                        yd + (2 + k / 4) * (kYBytes / 16) + 2 * (k % 4), id_s, k > 0 ? 1u : 0u);
           if (KV) {
             const uint32_t sb = sbase + kOffY + place(yd) + 4 * kYBytes;
-            tc_mma_f16(tmem + C::kDp, one_d, stat_desc(sb + 2 * C::kStatBytes), id_s, 1u);
-            tc_mma_f16(tmem + C::kD, one_d, stat_desc(sb + 3 * C::kStatBytes), id_d, 0u);
+            tc_mma_f16(tmem + C::kDp, one, stat_desc(sb + 2 * C::kStatBytes), id_s, 1u);
+            tc_mma_f16(tmem + C::kD, one, stat_desc(sb + 3 * C::kStatBytes), id_d, 0u);
           }
           tc_commit(dp_full0 + 8u * (j & 1));
         };

@@ -777,12 +777,12 @@ bool gn_ring(const GnParams& p) {
 }
 
 template <typename... P>
-cudaError_t gn_ring_smem(void (*kernel)(P...), size_t bytes) {
+cudaError_t gn_allow_smem(void (*kernel)(P...), size_t bytes) {
   return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
 }
 
 // Sequences up to this many bytes per CTA of a cluster of eight take one kernel.
-constexpr int64_t kGnClusterBytes = 64 * 1024;
+constexpr int64_t kGnClusterBytes = 128 * 1024;
 constexpr int kGnClusterMax = 8;
 
 template <typename T, int V, int GS>
@@ -803,8 +803,10 @@ sc_status gn_forward_v(Handle* h, GnParams p, const int32_t* cu, int batch) {
     // a rank for every eight rows of a row lane
     int ranks = 1;
     while (ranks < kGnClusterMax && longest > 8ll * ty * ranks) ranks *= 2;
-    e = launch_ex(h, k_gn_cluster<T, V, GS>, static_cast<int>(recs.size()) * ranks,
-                  gn_sum_smem(p.c, p.c / V) + sizeof(float) * 4 * p.groups, ranks, p, call.plan, ranks);
+    const size_t smem = gn_sum_smem(p.c, p.c / V) + sizeof(float) * 4 * p.groups;  // at most 96 KB
+    e = smem > 48 * 1024 ? gn_allow_smem(k_gn_cluster<T, V, GS>, smem) : cudaSuccess;
+    if (e == cudaSuccess)
+      e = launch_ex(h, k_gn_cluster<T, V, GS>, static_cast<int>(recs.size()) * ranks, smem, ranks, p, call.plan, ranks);
   } else {
     p.chunk = gn_chunk(h, cu, batch, p.c / V);
     sc_status st = gn_plan(h, cu, batch, p.chunk, &call);
@@ -819,8 +821,8 @@ sc_status gn_forward_v(Handle* h, GnParams p, const int32_t* cu, int batch) {
     ++h->launches;
     if (gn_ring<T, V>(p)) {
       if constexpr (V * sizeof(T) == 16) {
-        e = gn_ring_smem(k_gn_stats<T, V, true>, kGnRingSmem);
-        if (e == cudaSuccess) e = gn_ring_smem(k_gn_apply<T, V, GS, true>, kGnRingSmem + 2 * sizeof(float) * 4096);
+        e = gn_allow_smem(k_gn_stats<T, V, true>, kGnRingSmem);
+        if (e == cudaSuccess) e = gn_allow_smem(k_gn_apply<T, V, GS, true>, kGnRingSmem + 2 * sizeof(float) * 4096);
         if (e == cudaSuccess) {
           k_gn_stats<T, V, true><<<p.items, kGnThreads, kGnRingSmem, h->stream>>>(p, call.plan);
           e = launch_ex(h, k_gn_apply<T, V, GS, true>, p.items, kGnRingSmem + norms, 0, p, call.plan);
@@ -859,8 +861,8 @@ sc_status gn_backward_v(Handle* h, GnParams p, const int32_t* cu, int batch) {
   ++h->launches;
   if (gn_ring<T, V>(p)) {
     if constexpr (V * sizeof(T) == 16) {
-      e = gn_ring_smem(k_gn_bwd_sums<T, V, GS, true>, kGnRingSmem);
-      if (e == cudaSuccess) e = gn_ring_smem(k_gn_bwd_apply<T, V, GS, true>, kGnRingSmem + 2 * sizeof(float) * 4096);
+      e = gn_allow_smem(k_gn_bwd_sums<T, V, GS, true>, kGnRingSmem);
+      if (e == cudaSuccess) e = gn_allow_smem(k_gn_bwd_apply<T, V, GS, true>, kGnRingSmem + 2 * sizeof(float) * 4096);
       if (e == cudaSuccess) {
         k_gn_bwd_sums<T, V, GS, true><<<p.items, kGnThreads, kGnRingSmem, h->stream>>>(p, call.plan);
         e = launch_ex(h, k_gn_bwd_apply<T, V, GS, true>, dx_items + chan_ctas, kGnRingSmem + norms, 0, p, call.plan,

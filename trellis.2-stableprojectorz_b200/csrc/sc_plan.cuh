@@ -20,9 +20,10 @@ struct SeqRec {
   int32_t k0, k1;    // its key rows (attention)
   int32_t item0;     // first item
   int32_t aux;       // operator-specific
+  int32_t part0;     // first row of its partial results (attention)
 };
 
-constexpr int kPlanInline = 96;  // 2304 bytes of a kernel's 4 KB of parameters
+constexpr int kPlanInline = 96;  // 2688 bytes of a kernel's 4 KB of parameters
 
 struct SeqPlan {
   int32_t n = 0;                 // records
