@@ -252,6 +252,8 @@ def sparse_diff_attention(q, k, v, lam, cu_seqlens_q, cu_seqlens_kv=None, scale=
     defaults to the former); ``scale`` (2^-20 to 2^20) defaults to ``1 / sqrt(64)``.  With
     ``causal`` query i of a sequence sees the keys ``j <= i + len_kv - len_q``
     (a single new token sees the whole cache).  Rows that see no key are zero.
+    A NaN or an infinity stays inside its sequence; there it reaches rows that
+    ``causal`` hides it from too (0 * NaN), as in any product with the weights.
     Returns ``(total_N, H, 128)``.
 
     Differentiable in q, k, v and lam.  ``out`` receives the result without

@@ -527,7 +527,9 @@ sc_status run_forward(Handle* h, const DaArgs& a) {
   const uint32_t bq[4] = {kDaD, 1, static_cast<uint32_t>(p.pack), static_cast<uint32_t>(p.tokens)};
   const uint64_t rk = std::max<uint64_t>(static_cast<uint64_t>(nkv), one);
   const uint64_t dk[3] = {kDaD, 2ull * a.kv_heads, rk}, dv[3] = {kDaDv, static_cast<uint64_t>(a.kv_heads), rk};
-  const uint64_t sk[2] = {kDaD * 2, static_cast<uint64_t>(a.ks) * 2}, sv[2] = {kDaDv * 2, static_cast<uint64_t>(a.vs) * 2};
+  const uint64_t none = 128ull * a.kv_heads;  // without keys: any stride a map takes
+  const uint64_t sk[2] = {kDaD * 2, (nkv > 0 ? static_cast<uint64_t>(a.ks) : none) * 2},
+                 sv[2] = {kDaDv * 2, (nkv > 0 ? static_cast<uint64_t>(a.vs) : none) * 2};
   const uint32_t bk[3] = {kDaD, 1, kTile};
   // without keys no tile of them is read, but the maps want an address
   const void* k = nkv > 0 ? a.k : a.q;
