@@ -220,20 +220,20 @@ __device__ __forceinline__ void for_rows(int rows, const Place& at, L&& load, F&
   }
 }
 
-// The same rows through shared memory: blocks of 2 TY consecutive rows (at most
-// 16 KB; of two arrays: TY rows each) arrive by bulk copies in a ring of six, so
-// the bytes in flight cost no registers: 96 KB a CTA.  Dense rows of 16-byte
+// The same rows through shared memory: blocks of 4 TY consecutive rows (at most
+// 32 KB; of two arrays: 2 TY rows each) arrive by bulk copies in a ring of three,
+// so the bytes in flight cost no registers: 96 KB a CTA.  Dense rows of 16-byte
 // vectors only.  `last_first` walks the chunk's blocks from its end: the rows
 // that the pass before read last are the ones still in L2.  use(pack of array 0,
 // pack of array 1, row).
-constexpr int kGnRing = 6, kGnBlock = 16 * 1024, kGnRingSmem = kGnRing * kGnBlock + 16 * kGnRing + 128;
+constexpr int kGnRing = 3, kGnRows = 4, kGnBlock = kGnRows * 8 * 1024, kGnRingSmem = kGnRing * kGnBlock + 16 * kGnRing + 128;
 template <int ARRAYS, typename T, int V, typename F>
 __device__ __forceinline__ void ring_rows(const GnParams& p, const Chunk& ch, const Place& at, float* sm, const void* a0,
                                           const void* a1, bool last_first, F&& use) {
   const uint32_t base = (smem_u32(sm) + 127u) & ~127u;
   uint8_t* ring = reinterpret_cast<uint8_t*>(sm) + (base - smem_u32(sm));
   const uint32_t full0 = base + kGnRing * kGnBlock, empty0 = full0 + 8 * kGnRing;
-  const int row_bytes = p.c * static_cast<int>(sizeof(T)), per = (2 / ARRAYS) * at.TY;
+  const int row_bytes = p.c * static_cast<int>(sizeof(T)), per = kGnRows / ARRAYS * at.TY;
   const int blocks = (ch.rows + per - 1) / per;
   const char* src[2] = {static_cast<const char*>(a0) + ch.row0 * row_bytes,
                         static_cast<const char*>(a1) + ch.row0 * row_bytes};
@@ -266,7 +266,7 @@ __device__ __forceinline__ void ring_rows(const GnParams& p, const Chunk& ch, co
     const int b = last_first ? blocks - 1 - k : k, rows = min(per, ch.rows - b * per);
     if (at.live) {
 #pragma unroll
-      for (int u = 0; u < 2 / ARRAYS; ++u) {
+      for (int u = 0; u < kGnRows / ARRAYS; ++u) {
         const int r = at.ty + u * at.TY;
         if (r < rows) {
           Pack<T, V> v, g;
