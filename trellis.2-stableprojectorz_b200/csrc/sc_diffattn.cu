@@ -538,20 +538,16 @@ sc_status run_forward(Handle* h, const DaArgs& a) {
       !make_map_nd(&tv, bf16, v, 3, dv, sv, bk))
     return set_error(h, SC_ECUDA, "cuTensorMapEncodeTiled failed (differential attention)");
   SeqPlan plan;
-  void* table = nullptr;
-  sc_status st = make_plan(h, recs, &plan, &table);
+  DevBuf table(h), ws(h);
+  const sc_status st = make_plan(h, recs, &plan, &table.p);
   if (st != SC_OK) return st;
-  char* ws = nullptr;
   cudaError_t e = cudaSuccess;
   if (parts > 0) {
     const size_t n = static_cast<size_t>(parts) * a.heads;
-    e = dev_alloc(h, reinterpret_cast<void**>(&ws), n * (2 * kDaDv * sizeof(float) + sizeof(float4)));
-    if (e != cudaSuccess) {
-      dev_free(h, table);
-      return cuda_error(h, e, "differential attention workspace");
-    }
-    p.part_o = reinterpret_cast<float*>(ws);
-    p.part_ml = reinterpret_cast<float4*>(ws + n * 2 * kDaDv * sizeof(float));
+    e = dev_alloc(h, &ws.p, n * (2 * kDaDv * sizeof(float) + sizeof(float4)));
+    if (e != cudaSuccess) return cuda_error(h, e, "differential attention workspace");
+    p.part_o = static_cast<float*>(ws.p);
+    p.part_ml = reinterpret_cast<float4*>(static_cast<char*>(ws.p) + n * 2 * kDaDv * sizeof(float));
   }
   e = cudaFuncSetAttribute(k_da_fwd<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
   if (e == cudaSuccess) {
@@ -564,8 +560,6 @@ sc_status run_forward(Handle* h, const DaArgs& a) {
     }
     e = cudaGetLastError();
   }
-  dev_free(h, ws);
-  dev_free(h, table);
   return e == cudaSuccess ? SC_OK : cuda_error(h, e, "differential attention launch");
 }
 

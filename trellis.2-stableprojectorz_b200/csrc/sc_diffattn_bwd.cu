@@ -646,18 +646,16 @@ sc_status launch_bwd(Handle* h, const DaArgs& a, DaBwd p, const std::vector<int3
       !box_map(&mv, bf16, v, kDaDv, a.kv_heads, nkv, vs, KV ? kX : kY))
     return set_error(h, SC_ECUDA, "cuTensorMapEncodeTiled failed (differential attention backward)");
   SeqPlan plan;
-  void* table = nullptr;
-  const sc_status st = make_plan(h, recs, &plan, &table);
+  DevBuf table(h), part(h);
+  const sc_status st = make_plan(h, recs, &plan, &table.p);
   if (st != SC_OK) return st;
   cudaError_t e = cudaSuccess;
   p.nx = KV ? nkv : nq;
   const int wide = KV ? 256 : 128;
   if (splits > 1) {
-    e = dev_alloc(h, reinterpret_cast<void**>(&p.part), sizeof(float) * splits * p.nx * xheads * wide);
-    if (e != cudaSuccess) {
-      dev_free(h, table);
-      return cuda_error(h, e, "differential attention workspace");
-    }
+    e = dev_alloc(h, &part.p, sizeof(float) * splits * p.nx * xheads * wide);
+    if (e != cudaSuccess) return cuda_error(h, e, "differential attention workspace");
+    p.part = static_cast<float*>(part.p);
   }
   e = cudaFuncSetAttribute(k_da_bwd<T, KV>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<KV>::kSmem);
   if (e == cudaSuccess) {
@@ -674,8 +672,6 @@ sc_status launch_bwd(Handle* h, const DaArgs& a, DaBwd p, const std::vector<int3
     }
     e = cudaGetLastError();
   }
-  dev_free(h, p.part);
-  dev_free(h, table);
   return e == cudaSuccess ? SC_OK : cuda_error(h, e, "differential attention backward launch");
 }
 
@@ -712,18 +708,19 @@ sc_status run_backward(Handle* h, const DaArgs& a) {
   }
   p.np = rows + Cfg<true>::kY;  // a tile's copy may reach behind the last row
   const size_t per = static_cast<size_t>(a.heads) * p.np;
-  cudaError_t e = dev_alloc(h, reinterpret_cast<void**>(&p.split), per * (4 * sizeof(uint4) + 5 * sizeof(float)));
+  DevBuf buf(h);
+  cudaError_t e = dev_alloc(h, &buf.p, per * (4 * sizeof(uint4) + 5 * sizeof(float)));
+  p.split = static_cast<uint4*>(buf.p);
   if (e != cudaSuccess) return cuda_error(h, e, "differential attention workspace");
   p.st = reinterpret_cast<float*>(p.split + 4 * per);
   sc_status st = SC_OK;
   if (nq > 0) {
     SeqPlan plan;
-    void* table = nullptr;
-    st = make_plan(h, recs, &plan, &table);
+    DevBuf table(h);
+    st = make_plan(h, recs, &plan, &table.p);
     if (st == SC_OK) {
       ++h->launches;
       k_da_stats<T><<<static_cast<unsigned>((nq * a.heads + 7) / 8), 256, 0, h->stream>>>(p, plan);
-      dev_free(h, table);
     }
   }
   if (st == SC_OK && a.dlam) {
@@ -733,7 +730,6 @@ sc_status run_backward(Handle* h, const DaArgs& a) {
   if (st == SC_OK && (a.dk || a.dv)) st = launch_bwd<T, true>(h, a, p, st_row);
   if (st == SC_OK && a.dq) st = launch_bwd<T, false>(h, a, p, st_row);
   e = cudaGetLastError();
-  dev_free(h, p.split);
   if (st != SC_OK) return st;
   return e == cudaSuccess ? SC_OK : cuda_error(h, e, "differential attention backward launch");
 }

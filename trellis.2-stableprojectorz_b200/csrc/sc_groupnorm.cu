@@ -711,8 +711,9 @@ int gn_chunk(const Handle* h, const int32_t* cu, int batch, int nvec) {
 
 struct GnCall {
   SeqPlan plan;
-  void* table = nullptr;
+  DevBuf table, ws;
   int items = 0;
+  explicit GnCall(Handle* h) : table(h), ws(h) {}
 };
 
 sc_status gn_plan(Handle* h, const int32_t* cu, int batch, int chunk, GnCall* call) {
@@ -725,7 +726,7 @@ sc_status gn_plan(Handle* h, const int32_t* cu, int batch, int chunk, GnCall* ca
     items += (len + chunk - 1) / chunk;
   }
   call->items = static_cast<int>(items);
-  return make_plan(h, recs, &call->plan, &call->table);
+  return make_plan(h, recs, &call->plan, &call->table.p);
 }
 
 // Widest vector of T that divides the rows and their addresses.
@@ -791,14 +792,14 @@ sc_status gn_forward_v(Handle* h, GnParams p, const int32_t* cu, int batch) {
   for (int s = 0; s < batch; ++s) longest = std::max<int64_t>(longest, static_cast<int64_t>(cu[s + 1]) - cu[s]);
   const int64_t bytes = longest * p.c * static_cast<int64_t>(sizeof(T));
   const int ty = kGnThreads / std::min(p.c / V, kGnThreads);
-  GnCall call;
+  GnCall call(h);
   cudaError_t e;
   if (bytes <= kGnClusterMax * kGnClusterBytes) {
     std::vector<SeqRec> recs;
     for (int s = 0; s < batch; ++s)
       if (cu[s + 1] > cu[s])
         recs.push_back(SeqRec{cu[s], cu[s + 1], 0, 0, static_cast<int32_t>(recs.size()), s});
-    sc_status st = make_plan(h, recs, &call.plan, &call.table);
+    sc_status st = make_plan(h, recs, &call.plan, &call.table.p);
     if (st != SC_OK) return st;
     // a rank for every eight rows of a row lane
     int ranks = 1;
@@ -812,11 +813,9 @@ sc_status gn_forward_v(Handle* h, GnParams p, const int32_t* cu, int batch) {
     sc_status st = gn_plan(h, cu, batch, p.chunk, &call);
     if (st != SC_OK) return st;
     p.items = call.items;
-    e = dev_alloc(h, reinterpret_cast<void**>(&p.part), sizeof(float2) * p.groups * p.items);
-    if (e != cudaSuccess) {
-      dev_free(h, call.table);
-      return cuda_error(h, e, "group norm workspace");
-    }
+    e = dev_alloc(h, &call.ws.p, sizeof(float2) * p.groups * p.items);
+    if (e != cudaSuccess) return cuda_error(h, e, "group norm workspace");
+    p.part = static_cast<float2*>(call.ws.p);
     const size_t sums = gn_sum_smem(p.c, p.c / V), norms = sizeof(float) * 2 * p.groups;
     ++h->launches;
     if (gn_ring<T, V>(p)) {
@@ -834,27 +833,21 @@ sc_status gn_forward_v(Handle* h, GnParams p, const int32_t* cu, int batch) {
     }
   }
   if (e == cudaSuccess) e = cudaGetLastError();
-  dev_free(h, p.part);
-  dev_free(h, call.table);
   return e == cudaSuccess ? SC_OK : cuda_error(h, e, "group norm launch");
 }
 
 template <typename T, int V, int GS>
 sc_status gn_backward_v(Handle* h, GnParams p, const int32_t* cu, int batch) {
   p.chunk = gn_chunk(h, cu, batch, p.c / V);
-  GnCall call;
+  GnCall call(h);
   sc_status st = gn_plan(h, cu, batch, p.chunk, &call);
   if (st != SC_OK) return st;
   p.items = call.items;
   const size_t part = (sizeof(float2) * p.groups * p.items + 255) / 256 * 256;
-  char* ws = nullptr;
-  cudaError_t e = dev_alloc(h, reinterpret_cast<void**>(&ws), part + sizeof(float) * 2 * p.c * p.items);
-  if (e != cudaSuccess) {
-    dev_free(h, call.table);
-    return cuda_error(h, e, "group norm workspace");
-  }
-  p.part = reinterpret_cast<float2*>(ws);
-  p.chan = reinterpret_cast<float*>(ws + part);
+  cudaError_t e = dev_alloc(h, &call.ws.p, part + sizeof(float) * 2 * p.c * p.items);
+  if (e != cudaSuccess) return cuda_error(h, e, "group norm workspace");
+  p.part = static_cast<float2*>(call.ws.p);
+  p.chan = reinterpret_cast<float*>(static_cast<char*>(call.ws.p) + part);
   const int dx_items = p.dx ? p.items : 0;
   const int chan_ctas = p.dw || p.db ? (p.c + kGnChanBlock - 1) / kGnChanBlock : 0;
   const size_t sums = gn_sum_smem(p.c, p.c / V), norms = sizeof(float) * 2 * std::max(p.groups, kGnThreads);
@@ -874,8 +867,6 @@ sc_status gn_backward_v(Handle* h, GnParams p, const int32_t* cu, int batch) {
     e = launch_ex(h, k_gn_bwd_apply<T, V, GS, false>, dx_items + chan_ctas, norms, 0, p, call.plan, chan_ctas);
   }
   if (e == cudaSuccess) e = cudaGetLastError();
-  dev_free(h, ws);
-  dev_free(h, call.table);
   return e == cudaSuccess ? SC_OK : cuda_error(h, e, "group norm backward launch");
 }
 

@@ -74,6 +74,17 @@ struct KMap {
 cudaError_t dev_alloc(Handle* h, void** p, size_t bytes);
 void dev_free(Handle* h, void* p);
 
+// Stream-ordered device memory freed with its scope (also when a host
+// allocation throws).
+struct DevBuf {
+  Handle* h;
+  void* p = nullptr;
+  explicit DevBuf(Handle* handle) : h(handle) {}
+  DevBuf(const DevBuf&) = delete;
+  DevBuf& operator=(const DevBuf&) = delete;
+  ~DevBuf() { dev_free(h, p); }
+};
+
 // Per-axis dilation of a 3x3x3 kernel (dilD on x, dilH on y, dilW on z).
 struct Dil {
   int x, y, z;

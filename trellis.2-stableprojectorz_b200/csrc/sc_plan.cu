@@ -39,11 +39,7 @@ sc_status make_plan(Handle* h, const std::vector<SeqRec>& recs, SeqPlan* plan, v
     k_plan_write<<<1, kPlanInline, 0, h->stream>>>(c, d + at);
   }
   const cudaError_t le = cudaGetLastError();
-  if (le != cudaSuccess) {
-    dev_free(h, *dev);
-    *dev = nullptr;
-    return cuda_error(h, le, "sequence table");
-  }
+  if (le != cudaSuccess) return cuda_error(h, le, "sequence table");
   plan->ext = d;
   return SC_OK;
 }

@@ -42,8 +42,8 @@ struct SeqPlan {
 };
 
 // Fills `plan` from host records (no record may have zero items).  *dev
-// receives the device table, if one was needed, for dev_free after the
-// call's last kernel.
+// receives the device table, if one was needed; the caller frees it behind its
+// last kernel, also after an error.
 sc_status make_plan(Handle* h, const std::vector<SeqRec>& recs, SeqPlan* plan, void** dev);  // sc_plan.cu
 
 }  // namespace sc
