@@ -62,7 +62,7 @@ struct DaFwd {
   int64_t nq;
   int heads, rep, pack, tokens;  // rep = heads / kv_heads; heads and tokens of a tile (pack * tokens rows)
   int causal;
-  int split_keys;   // keys per range, a multiple of 128
+  int split_keys;   // keys per range (the last may be short and fills gaps), a multiple of 128
   float scale_log2;
   int* err;
 };
@@ -98,6 +98,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t s_full0 = kv_empty0 + 8 * kStages, p_full0 = s_full0 + 16, o_done0 = p_full0 + 16;  // per map
   const uint32_t s_free = o_done0 + 16, done_bar = s_free + 8, v_req = done_bar + 8, v_fixed = v_req + 8;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const SeqRec& rec = plan.at(plan.find(blockIdx.x));
   const DaTile tile(rec, blockIdx.x - rec.item0, p);
   const int g = blockIdx.y, h0 = g * p.pack;
@@ -105,7 +106,18 @@ __global__ void __launch_bounds__(kThreads, 1)
   const bool last_partial = nk > 0 && tile.key1 - tile.key0 < nk * kTile;
   const int rows = tile.ntok * p.pack;
 
-  if (threadIdx.x == 0) {
+  const int gk = h0 / p.rep;  // key / value head
+  auto load_tile = [&](int j) {
+    const uint32_t kb = sbase + kOffKV + (j % kStages) * kStageBytes, bar = kv_full0 + 8 * (j % kStages);
+    const int row = rec.k0 + tile.key0 + j * kTile;
+    mbar_arrive_expect_tx(bar, kStageBytes);
+    tma_load_3d(kb, &tmK, 0, 2 * gk, row, bar);
+    tma_load_3d(kb + kQBytes, &tmK, 0, 2 * gk + 1, row, bar);
+    tma_load_3d(kb + 2 * kQBytes, &tmV, 0, gk, row, bar);
+    tma_load_3d(kb + 3 * kQBytes, &tmV, 64, gk, row, bar);
+  };
+  // the barriers, and at once the loads that wait for nothing
+  if (warp == 0 && elect_one()) {
     mbar_init(q_full, 1);
     for (int st = 0; st < kStages; ++st) {
       mbar_init(kv_full0 + 8 * st, 1);
@@ -121,7 +133,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     mbar_init(v_req, 1);
     mbar_init(v_fixed, 1);
     fence_mbar_init();
+    if (nk > 0) {
+      mbar_arrive_expect_tx(q_full, 2 * p.pack * p.tokens * 128);
+      for (int m = 0; m < 2; ++m)
+        tma_load_4d(sbase + kOffQ + m * kQBytes, &tmQ, 0, m, h0, rec.q0 + tile.tok0, q_full);
+      for (int j = 0; j < min(nk, kStages); ++j) load_tile(j);
+    }
   }
+  __syncwarp();
   if (warp == 1) {
     tmem_alloc(smem_u32(s_tmem), kTmem);
     tmem_relinquish();
@@ -136,20 +155,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (warp == 0) {
     // ----------------------------------------------------------- producer
     if (nk > 0 && elect_one()) {
-      const int gk = h0 / p.rep;
-      mbar_arrive_expect_tx(q_full, 2 * p.pack * p.tokens * 128);
-      for (int m = 0; m < 2; ++m)
-        tma_load_4d(sbase + kOffQ + m * kQBytes, &tmQ, 0, m, h0, rec.q0 + tile.tok0, q_full);
-      for (int j = 0; j < nk; ++j) {
-        const int st = j % kStages;
-        if (!mbar_wait(kv_empty0 + 8 * st, ((j / kStages) & 1) ^ 1, p.err)) break;
-        const uint32_t kb = sbase + kOffKV + st * kStageBytes, bar = kv_full0 + 8 * st;
-        const int row = rec.k0 + tile.key0 + j * kTile;
-        mbar_arrive_expect_tx(bar, kStageBytes);
-        tma_load_3d(kb, &tmK, 0, 2 * gk, row, bar);
-        tma_load_3d(kb + kQBytes, &tmK, 0, 2 * gk + 1, row, bar);
-        tma_load_3d(kb + 2 * kQBytes, &tmV, 0, gk, row, bar);
-        tma_load_3d(kb + 3 * kQBytes, &tmV, 64, gk, row, bar);
+      for (int j = kStages; j < nk; ++j) {
+        if (!mbar_wait(kv_empty0 + 8 * (j % kStages), ((j / kStages) & 1) ^ 1, p.err)) break;
+        load_tile(j);
       }
     }
   } else if (warp == 1) {
@@ -391,6 +399,7 @@ __global__ void __launch_bounds__(128) k_da_join(const DaFwd p, const __grid_con
   const int lane = threadIdx.x & 31;
   if (at >= p.nq * p.heads) return;
   const int row = static_cast<int>(at / p.heads), h = static_cast<int>(at % p.heads);
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // launched before k_da_fwd ends
   int rec = 0;
   for (int base = 0; base < nrec; base += 32) {  // records are sorted by key count, not by row
     const int i = base + lane;
@@ -555,10 +564,18 @@ sc_status run_forward(Handle* h, const DaArgs& a) {
     k_da_fwd<T><<<dim3(static_cast<unsigned>(items), groups), kThreads, kSmem, h->stream>>>(tq, tk, tv, p, plan);
     if (parts > 0) {
       ++h->launches;
-      k_da_join<T><<<static_cast<unsigned>((nq * a.heads + 3) / 4), 128, 0, h->stream>>>(
-          p, plan, static_cast<int>(recs.size()));
+      cudaLaunchConfig_t cfg{};
+      cfg.gridDim = dim3(static_cast<unsigned>((nq * a.heads + 3) / 4));
+      cfg.blockDim = dim3(128);
+      cfg.stream = h->stream;
+      cudaLaunchAttribute at[1];
+      at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+      at[0].val.programmaticStreamSerializationAllowed = 1;
+      cfg.attrs = at;
+      cfg.numAttrs = 1;
+      e = cudaLaunchKernelEx(&cfg, k_da_join<T>, p, plan, static_cast<int>(recs.size()));
     }
-    e = cudaGetLastError();
+    if (e == cudaSuccess) e = cudaGetLastError();
   }
   return e == cudaSuccess ? SC_OK : cuda_error(h, e, "differential attention launch");
 }
