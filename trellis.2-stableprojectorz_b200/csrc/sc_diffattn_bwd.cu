@@ -58,8 +58,8 @@ struct Cfg {
   // Y_1, Y_2, halves of the 128-wide one; statistics: 16-byte rows for S_1, S_2
   // and dP (kY each) and of delta_1 - delta_2 (kDiff), and the rest of it in f32
   static constexpr int kDiff = 32, kStatBytes = 16 * kY, kDiffBytes = 16 * kDiff, kRestBytes = 4 * (kY - kDiff);
-  static constexpr int kStage = 4 * kYBytes + (KV ? 3072 : 0);
-  static_assert(3 * kStatBytes + kDiffBytes + kRestBytes <= 3072, "stage");
+  static constexpr int kStage = 4 * kYBytes + (KV ? 3 * 1024 : 0);
+  static_assert(3 * kStatBytes + kDiffBytes + kRestBytes <= 3 * 1024, "stage");
   // constant rows against the split statistics (128 of 16 bytes), and zeros
   static constexpr int kOffOnes = kOffY + kStages * kStage, kOffZero = kOffOnes + kX * 16;
   static constexpr int kOffBar = kOffZero + kX * 16;
