@@ -158,10 +158,15 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (warp == 0) {
     // ----------------------------------------------------------- producer
     if (nk > 0 && elect_one()) {
-      for (int j = kStages; j < nk; ++j) {
+      int j = min(nk, kStages);
+      for (; j < nk; ++j) {
         if (!mbar_wait(kv_empty0 + 8 * (j % kStages), ((j / kStages) & 1) ^ 1, p.err)) break;
         load_tile(j);
       }
+      // the copies end before the CTA does, also where a wait has given up
+      mbar_wait(q_full, 0, p.err);
+      for (int i = max(0, j - kStages); i < j; ++i)
+        mbar_wait(kv_full0 + 8 * (i % kStages), (i / kStages) & 1, p.err);
     }
   } else if (warp == 1) {
     // ---------------------------------------------------------- MMA issuer

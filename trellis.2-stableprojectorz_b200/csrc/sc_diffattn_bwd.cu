@@ -256,8 +256,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         tma_load_3d(sbase + kOffX + kXBytes, &tmX, 0, 2 * xh + 1, xrow, x_full);
         tma_load_3d(sbase + kOffX + 2 * kXBytes, &tmXw, 0, xh, xrow, x_full);
         tma_load_3d(sbase + kOffX + 3 * kXBytes, &tmXw, 64, xh, xrow, x_full);
-        int ty = t0 % ny, yh = KV ? g * p.rep + t0 / ny : g, st = 0, use = 0;
-        for (int j = 0; j < n; ++j) {
+        int ty = t0 % ny, yh = KV ? g * p.rep + t0 / ny : g, st = 0, use = 0, j = 0;
+        for (; j < n; ++j) {
           if (!mbar_wait(y_empty0 + 8 * st, (use & 1) ^ 1, p.err)) break;
           const uint32_t yb = sbase + kOffY + st * C::kStage, bar = y_full0 + 8 * st;
           const int yr = y0 + ty * kY, yrow = (KV ? rec.q0 : rec.k0) + yr;
@@ -276,6 +276,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (++ty == ny) ty = 0, yh += KV ? 1 : 0;
           if (++st == kStages) st = 0, ++use;
         }
+        // the copies end before the CTA does, also where a wait has given up
+        mbar_wait(x_full, 0, p.err);
+        for (int i = max(0, j - kStages); i < j; ++i) mbar_wait(y_full0 + 8 * (i % kStages), (i / kStages) & 1, p.err);
       }
     } else if (warp == 1) {
       // ------------------------------------------------- S and dP of every step
