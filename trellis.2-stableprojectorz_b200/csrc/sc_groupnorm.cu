@@ -253,16 +253,18 @@ __device__ __forceinline__ void ring_rows(const GnParams& p, const Chunk& ch, co
       bulk_load(base + s * kGnBlock + i * (kGnBlock / 2), src[i] + static_cast<int64_t>(b) * per * row_bytes, bytes,
                 full0 + 8 * s);
   };
+  int issued = min(blocks, kGnRing - 1);  // thread 0's
   if (threadIdx.x == 0)
-    for (int k = 0; k < min(blocks, kGnRing - 1); ++k) issue(k);
-  int s = 0, turn = 0;
-  for (int k = 0; k < blocks; ++k) {
-    if (threadIdx.x == 0 && k + kGnRing - 1 < blocks) {
-      // the slot of block k - 1, once every warp has left it
-      if (k == 0 || mbar_wait(empty0 + 8 * ((k - 1) % kGnRing), ((k - 1) / kGnRing) & 1, p.err)) issue(k + kGnRing - 1);
+    for (int k = 0; k < issued; ++k) issue(k);
+  int s = 0, turn = 0, k = 0;
+  for (; k < blocks; ++k) {
+    if (threadIdx.x == 0 && issued < blocks && issued == k + kGnRing - 1) {
+      // the slot of block k - 1, once every warp has left it; none is asked for after a wait that gave up
+      if (k == 0 || mbar_wait(empty0 + 8 * ((k - 1) % kGnRing), ((k - 1) / kGnRing) & 1, p.err)) issue(issued++);
     }
     __syncwarp();
-    if (!mbar_wait(full0 + 8 * s, turn, p.err)) break;
+    // a warp goes on or leaves as one: its lanes meet again below
+    if (!__all_sync(0xffffffffu, mbar_wait(full0 + 8 * s, turn, p.err))) break;
     const int b = last_first ? blocks - 1 - k : k, rows = min(per, ch.rows - b * per);
     if (at.live) {
 #pragma unroll
@@ -280,6 +282,9 @@ __device__ __forceinline__ void ring_rows(const GnParams& p, const Chunk& ch, co
     if ((threadIdx.x & 31) == 0) mbar_arrive(empty0 + 8 * s);
     if (++s == kGnRing) s = 0, turn ^= 1;
   }
+  // after a wait that gave up: the copies end before sm is used again
+  if (threadIdx.x == 0)
+    for (; k < issued; ++k) mbar_wait(full0 + 8 * (k % kGnRing), (k / kGnRing) & 1, p.err);
   __syncthreads();  // sm may be used again
 }
 
