@@ -1,5 +1,7 @@
 """Group norm and differential attention without a GPU: the restatements'
 gradients against differences, and what the calls refuse."""
+import ctypes
+
 import numpy as np
 import pytest
 import torch
@@ -97,6 +99,39 @@ def test_group_norm_refusals(pkg):
             f(x, 4, eps=eps)
     with pytest.raises(ValueError, match="end at"):
         f(x, 4, cu_seqlens=[0, 5])
+
+
+class _Recorder:
+    """An engine that keeps what its calls pass: the values behind the given arguments, read as dense f32."""
+
+    def __init__(self, count, at):
+        self.count, self.at, self.seen = count, at, []
+
+    def call(self, name, *args):
+        read = lambda p: np.ctypeslib.as_array((ctypes.c_float * self.count).from_address(p)).copy()  # noqa: E731
+        self.seen.append((name, *(None if args[i] is None else read(args[i]) for i in self.at[name])))
+
+
+@pytest.mark.parametrize("grad", [False, True])
+def test_group_norm_passes_dense_weights(pkg, monkeypatch, grad):
+    """The library reads C consecutive values of weight and bias, so strided and expanded ones are copied, in both
+    directions.  (Their storages hold more than C values: the reads here stay in range whatever is passed.)"""
+    ops, c = pkg.block_ops, 8
+    x, dy = torch.randn(6, c), torch.ones(6, c)
+    table = torch.randn(2 * c, 3)
+    w, b = table[:c, 1], table.view(-1)[4:5].expand(c)
+    engine = _Recorder(c, {"sc_group_norm": (2, 3), "sc_group_norm_backward": (3, 4)})
+    monkeypatch.setattr(ops, "get_engine", lambda device: engine)
+    cu = ops._offsets([0, 6], 6, "cu")
+    if grad:
+        leaves = [t.detach().requires_grad_() for t in (x, w, b)]
+        torch.autograd.grad(ops._GroupNorm.apply(*leaves, 4, 1e-5, cu, True), leaves, dy)
+    else:
+        ops._gn_forward(x, 4, w, b, 1e-5, cu, True, None, False)
+    assert [s[0] for s in engine.seen] == ["sc_group_norm", "sc_group_norm_backward"][:1 + grad]
+    for _, gw, gb in engine.seen:
+        np.testing.assert_array_equal(gw, w.numpy())
+        np.testing.assert_array_equal(gb, b.numpy())
 
 
 def test_diff_attention_refusals(pkg):

@@ -142,6 +142,26 @@ def test_group_norm_rows_apart_and_in_place(pkg, cuda):
         pkg.sparse_group_norm(xc, 16, w, b, out=xc.float())
 
 
+@pytest.mark.parametrize("dtype", [FP, BF])
+def test_group_norm_weights_apart(pkg, cuda, dtype):
+    """A column of a table and an expanded single value as weight or bias, with and without gradients: as the dense ones."""
+    x, w, b, dy = _gn_inputs(cuda, 333, 64, dtype, FP, 12)
+    table = torch.stack((b, w, b), 1)
+    col, one = table[:, 1], w[5:6].expand(64)
+    for weight, bias in ((col, one), (one, table[:, 0]), (col, None), (None, one)):
+        dense = [None if t is None else t.contiguous() for t in (weight, bias)]
+        ref = pkg.sparse_group_norm(x, 16, *dense, silu=True)
+        assert torch.equal(pkg.sparse_group_norm(x, 16, weight, bias, silu=True), ref)
+        given = []
+        for pair in (dense, (weight, bias)):
+            leaves = [t.detach().requires_grad_() for t in (x, *pair) if t is not None]
+            vectors = iter(leaves[1:])
+            y = pkg.sparse_group_norm(leaves[0], 16, *(None if t is None else next(vectors) for t in pair), silu=True)
+            given.append((y, *torch.autograd.grad(y, leaves, dy)))
+        assert torch.equal(given[0][0], ref)
+        assert all(torch.equal(p, r) for p, r in zip(*given))
+
+
 def test_group_norm_of_nothing(pkg, cuda):
     x = torch.zeros(0, 32, device=cuda, dtype=BF, requires_grad=True)
     w = torch.ones(32, device=cuda, requires_grad=True)

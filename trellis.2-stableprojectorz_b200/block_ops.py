@@ -88,8 +88,14 @@ def _rows_view(x):
 
 
 # ------------------------------------------------------------------ group norm
+def _dense_vectors(*vectors):
+    """The library reads ``(C,)`` consecutive values: strided and expanded vectors are copied."""
+    return tuple(None if t is None else t.contiguous() for t in vectors)
+
+
 def _gn_forward(x, groups, weight, bias, eps, cu, silu, out, want_stats):
     x, stride = _rows_view(x)
+    weight, bias = _dense_vectors(weight, bias)
     wd = _DTYPES[(weight if weight is not None else bias if bias is not None else x).dtype]
     y = _dense(x) if out is None else out
     stats = torch.empty((len(cu) - 1, groups, 2), dtype=torch.float32, device=x.device) if want_stats else None
@@ -118,8 +124,7 @@ class _GroupNorm(torch.autograd.Function):
         dw = _dense(weight) if need_w else None
         db = _dense(bias) if need_b else None
         wd = _DTYPES[(weight if weight is not None else bias if bias is not None else x).dtype]
-        weight = None if weight is None else weight.contiguous()
-        bias = None if bias is None else bias.contiguous()
+        weight, bias = _dense_vectors(weight, bias)
         get_engine(x.device).call("sc_group_norm_backward", _p(x), stride, _p(dy), _p(weight), _p(bias), _p(stats),
                                   _p(dx), _p(dw), _p(db), cu, len(cu) - 1, x.shape[1], groups, int(silu),
                                   _DTYPES[x.dtype], wd)
@@ -173,8 +178,6 @@ def sparse_group_norm(x, num_groups, weight=None, bias=None, eps=1e-5, cu_seqlen
         same = out.data_ptr() == x.data_ptr() and x.is_contiguous()
         if (_overlap(out, x) and not same) or _overlap(out, weight) or _overlap(out, bias):
             raise ValueError("out overlaps an input (only a contiguous x itself may be written in place)")
-    weight = None if weight is None else weight.contiguous()
-    bias = None if bias is None else bias.contiguous()
     return _gn_forward(x, groups, weight, bias, eps, cu, silu, out, False)[0]
 
 
