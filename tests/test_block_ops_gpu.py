@@ -371,6 +371,69 @@ def test_diff_attention_sequences_stay_isolated(pkg, cuda):
         assert torch.equal(a[:200], b[:200])
 
 
+def _da_plain(q, k, v, lam, cu_q, cu_kv):
+    """Float64, no mask; torch's own rules for NaN and infinities."""
+    q, k, v, lam = (t.detach().double().cpu() for t in (q, k, v, lam))
+    out = torch.zeros(q.shape[0], q.shape[1] // 2, 128, dtype=torch.float64)
+    rep = out.shape[1] // v.shape[1]
+    for a, b, c, d in zip(cu_q, cu_q[1:], cu_kv, cu_kv[1:]):
+        for h in range(out.shape[1] if b > a and d > c else 0):
+            g = h // rep
+            m = [torch.softmax(q[a:b, 2 * h + i] @ k[c:d, 2 * g + i].T / 8, -1) @ v[c:d, g] for i in (0, 1)]
+            out[a:b, h] = m[0] - lam[h] * m[1]
+    return out
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("train", [False, True])
+@pytest.mark.parametrize("cu_q,cu_kv", [([0, 150, 300], [0, 200, 500]),  # whole sequences
+                                        ([0, 1, 2], [0, 700, 5700])])    # keys cut into ranges
+@pytest.mark.parametrize("where", ["q", "q1", "k", "v"])
+@pytest.mark.parametrize("bad", ["nan", "inf", "-inf"])
+def test_diff_attention_nan_and_infinity_reach_their_rows(pkg, cuda, dtype, train, cu_q, cu_kv, where, bad):
+    """A NaN or an infinity in a sequence makes the values non-finite that it makes non-finite in float64, and no
+    others; the rest is as close as ever (a score of -inf is a weight of 0).  lse goes with its map."""
+    q, k, v, lam, _ = _da_inputs(cuda, cu_q[-1], cu_kv[-1], 4, 2, dtype, 50)
+    {"q": q[cu_q[1]], "q1": q[cu_q[1], 1], "k": k[cu_kv[1] + 130], "v": v[cu_kv[1] + 130]}[where][..., 5] = float(bad)
+    q.requires_grad_(train)
+    got = pkg.sparse_diff_attention(q, k, v, lam, cu_q, cu_kv)
+    ref = _da_plain(q, k, v, lam, cu_q, cu_kv)
+    fin = ref.isfinite()
+    assert not fin.all()
+    if where == "v":  # the maps' difference of infinities is NaN, as is 0 * inf of a weight that underflows
+        assert not fin[cu_q[1]:, :, 5].any()
+    out = got.detach().double().cpu()
+    assert torch.equal(out.isfinite(), fin)
+    assert _rel(out[fin].numpy(), ref[fin].numpy()) < 2 * _half(dtype) + 2e-4
+    if train:
+        lse = got.grad_fn.saved_tensors[5]  # [2][heads][rows]
+        maps = got.grad_fn.saved_tensors[4]
+        if where == "v":
+            assert lse.isfinite().all()
+        else:
+            assert torch.equal(lse.isnan(), maps.isnan().all(3).permute(2, 1, 0))
+            assert lse.isnan().any() and not lse.isinf().any()
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_diff_attention_without_a_softmax(pkg, cuda, dtype):
+    """Scores that are all -inf have no softmax: NaN, for whole sequences and for joined ranges; without keys a row
+    stays zero whatever its query holds."""
+    for cu_kv in ([0, 3, 203, 203], [0, 700, 5700, 5700]):
+        cu_q = [0, 1, 2, 4]
+        q, k, v, lam, _ = _da_inputs(cuda, 4, cu_kv[-1], 2, 1, dtype, 51)
+        k[:cu_kv[1], :, 9] = -1.0
+        q[0, :, 9] = float("inf")
+        q[2:] = float("nan")
+        for train in (False, True):
+            out = pkg.sparse_diff_attention(q.requires_grad_(train), k, v, lam, cu_q, cu_kv)
+            assert out[0].isnan().all() and out[1].isfinite().all() and torch.count_nonzero(out[2:]) == 0
+            if train:
+                lse = out.grad_fn.saved_tensors[5]
+                assert lse[..., 0].isnan().all() and lse[..., 1].isfinite().all() and (lse[..., 2:] == np.inf).all()
+            q = q.detach()
+
+
 def test_diff_attention_past_32_bit_offsets(pkg, cuda):
     """A cache whose last sequence lies past 2^31 elements of k and v."""
     n, hk = 2_150_000, 8

@@ -343,13 +343,16 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int64_t at = live ? qrow * p.heads + head : 0;
       const bool join = tile.nsplit > 1;
       const int64_t part = (rec.part0 + static_cast<int64_t>(tile.split) * (rec.q1 - rec.q0) + tok) * p.heads + head;
-      const float i1 = r1.y > 0.f ? 1.f / r1.y : 0.f, i2 = r2.y > 0.f ? 1.f / r2.y : 0.f;
+      // a sum of 0: no key, or scores of -inf alone, which have no softmax; a NaN sum goes through
+      const float none = live && !join && key_limit(rec, tok, p.causal) > 0 ? NAN : 0.f;
+      const float i1 = join ? 1.f : 1.f / r1.y, i2 = join ? 1.f : 1.f / r2.y;
       const float lam = live ? p.lam.get(head) : 0.f;
       if (live && join && m == 0)
         p.part_ml[part] = make_float4(r1.x, r1.y, r2.x, r2.y);
       if (live && !join && p.lse) {
         const float2 r = m ? r2 : r1;
-        p.lse[(static_cast<int64_t>(m) * p.heads + head) * p.nq + qrow] = r.y > 0.f ? r.x + log2f(r.y) : INFINITY;
+        p.lse[(static_cast<int64_t>(m) * p.heads + head) * p.nq + qrow] =
+            r.y != 0.f ? r.x + log2f(r.y) : none != 0.f ? NAN : INFINITY;
       }
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
@@ -360,11 +363,11 @@ __global__ void __launch_bounds__(kThreads, 1)
           tmem_ld32(lane_base + kColO + 128u + 64u * m + 32u * c, o2);
         }
         const int d = 64 * m + 32 * c;
-        // a map without a sum has no product: its columns were never written
+        // without a sum the columns may never have been written
 #pragma unroll
         for (int i = 0; i < 32; ++i) {
-          o1[i] = r1.y > 0.f ? o1[i] * (join ? 1.f : i1) : 0.f;
-          o2[i] = r2.y > 0.f ? o2[i] * (join ? 1.f : i2) : 0.f;
+          o1[i] = r1.y != 0.f ? o1[i] * i1 : none;
+          o2[i] = r2.y != 0.f ? o2[i] * i2 : none;
         }
         float* f32 = join ? p.part_o + part * (2 * kDaDv) : p.maps ? p.maps + at * (2 * kDaDv) : nullptr;
         if (live && f32) {
@@ -435,7 +438,8 @@ __global__ void __launch_bounds__(128) k_da_join(const DaFwd p, const __grid_con
     }
     const float n1 = fmaxf(m1, t1), n2 = fmaxf(m2, t2);
     const float a1 = m1 > -INFINITY ? exp2f(m1 - n1) : 0.f, a2 = m2 > -INFINITY ? exp2f(m2 - n2) : 0.f;
-    const float w1 = ml.y > 0.f ? exp2f(ml.x - n1) : 0.f, w2 = ml.w > 0.f ? exp2f(ml.z - n2) : 0.f;
+    // a range without a sum has weight 0; a NaN sum goes through
+    const float w1 = ml.y != 0.f ? exp2f(ml.x - n1) : 0.f, w2 = ml.w != 0.f ? exp2f(ml.z - n2) : 0.f;
     float s1 = w1 * ml.y, s2 = w2 * ml.w;
 #pragma unroll
     for (int x = 16; x > 0; x >>= 1) {
@@ -464,15 +468,19 @@ __global__ void __launch_bounds__(128) k_da_join(const DaFwd p, const __grid_con
       }
     }
   }
-  const float i1 = l1 > 0.f ? 1.f / l1 : 0.f, i2 = l2 > 0.f ? 1.f / l2 : 0.f, lam = p.lam.get(h);
+  // a sum of 0: no key, or scores of -inf alone, which have no softmax
+  const float none = key_limit(r, row - r.q0, p.causal) > 0 ? NAN : 0.f;
+  const float i1 = l1 != 0.f ? 1.f / l1 : none, i2 = l2 != 0.f ? 1.f / l2 : none, lam = p.lam.get(h);
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
     o1[e] *= i1;
     o2[e] *= i2;
   }
-  if (p.lse && lane < 2)
+  if (p.lse && lane < 2) {
+    const float l = lane ? l2 : l1;
     p.lse[(static_cast<int64_t>(lane) * p.heads + h) * p.nq + row] =
-        (lane ? l2 : l1) > 0.f ? (lane ? m2 + log2f(l2) : m1 + log2f(l1)) : INFINITY;
+        l != 0.f ? (lane ? m2 : m1) + log2f(l) : none != 0.f ? NAN : INFINITY;
+  }
   if (p.maps) {
     float* dst = p.maps + at * (2 * kDaDv) + 4 * lane;
     *reinterpret_cast<float4*>(dst) = make_float4(o1[0], o1[1], o1[2], o1[3]);

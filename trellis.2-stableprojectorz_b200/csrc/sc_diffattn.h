@@ -19,7 +19,8 @@ struct DaArgs {
   int lam_dtype;
   float lam_value;
   void* out;              // [Nq, heads, 128]
-  float* lse;             // [2][heads][Nq] or null: log2 sum 2^(s log2 e) of every row and map, +inf without keys
+  float* lse;             // [2][heads][Nq] or null: log2 sum 2^(s log2 e) of every row and map, +inf without
+                          // keys, NaN where a score is NaN or +inf or every one is -inf
   float* maps;            // [Nq, heads, 2, 128] or null: O_1 and O_2 of every row.  f32: dO . O_m is subtracted from
                           // every score gradient of its row, and with O_m rounded to bf16 that one error, common to
                           // the row's keys, made up most of dq's (0.0039 relative at 8,192 keys, 0.0017 without)
