@@ -416,6 +416,45 @@ def test_diff_attention_nan_and_infinity_reach_their_rows(pkg, cuda, dtype, trai
 
 
 @pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("where", ["q", "q1", "k", "v", "dout"])
+@pytest.mark.parametrize("bad", ["nan", "inf"])
+def test_diff_attention_nan_and_infinity_reach_their_gradients(pkg, cuda, dtype, where, bad):
+    """Every gradient that float64 makes non-finite is non-finite; another sequence's are untouched."""
+    cu_q, cu_kv, heads = [0, 150, 300], [0, 200, 500], 4
+    q, k, v, lam, dout = _da_inputs(cuda, 300, 500, heads, 2, dtype, 52)
+    leaves = [t.requires_grad_() for t in (q, k, v, lam)]
+    clean = torch.autograd.grad(pkg.sparse_diff_attention(*leaves, cu_q, cu_kv), leaves, dout)
+    with torch.no_grad():
+        {"q": q[170], "q1": q[170, 1], "k": k[330], "v": v[330], "dout": dout[170]}[where][..., 5] = float(bad)
+    got = torch.autograd.grad(pkg.sparse_diff_attention(*leaves, cu_q, cu_kv), leaves, dout)
+    given = [t.detach().double().cpu().requires_grad_() for t in leaves]
+    parts = []
+    for a, b, c, d in zip(cu_q, cu_q[1:], cu_kv, cu_kv[1:]):
+        hs = []
+        for h in range(heads):
+            m = [torch.softmax(given[0][a:b, 2 * h + i] @ given[1][c:d, 2 * (h // 2) + i].T / 8, -1) for i in (0, 1)]
+            hs.append((m[0] - given[3][h] * m[1]) @ given[2][c:d, h // 2])
+        parts.append(torch.stack(hs, 1))
+    ref = torch.autograd.grad(torch.cat(parts), given, dout.double().cpu())
+    for name, g, r, was, first in zip(("q", "k", "v", "lam"), got, ref, clean, (150, 200, 200, 0)):
+        fin = g.isfinite().cpu()
+        assert not (fin & ~r.isfinite()).any(), (name, int((fin & ~r.isfinite()).sum()))
+        assert torch.equal(g[:first], was[:first])
+
+
+def test_diff_attention_scores_past_the_f16_statistics(pkg, cuda):
+    """f16 scores of 7.1e7 before the scale: the backward says NaN where it can not hold the row's log-sum-exp."""
+    q = torch.full((40, 2, 64), 1050.0, dtype=HF, device=cuda)
+    k, v, dout = q.clone(), torch.randn(40, 1, 128, device=cuda).to(HF), torch.randn(40, 1, 128, device=cuda).to(HF)
+    k[7:] *= -1
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+    out = pkg.sparse_diff_attention(*leaves, 0.5, [0, 40], scale=2.0 ** -20)
+    assert out.isfinite().all()
+    for g in torch.autograd.grad(out, leaves, dout)[1:]:
+        assert g.isnan().any()
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
 def test_diff_attention_without_a_softmax(pkg, cuda, dtype):
     """Scores that are all -inf have no softmax: NaN, for whole sequences and for joined ranges; without keys a row
     stays zero whatever its query holds."""

@@ -102,7 +102,9 @@ __device__ __forceinline__ unsigned long long mul_f2(unsigned long long a, unsig
   return d;
 }
 // A statistic v as three values of T, v = k0 a + k1 b + k2 c.  bf16 has f32's
-// range.  f16: up to 65,504 * 1,024, in steps of 2^-34.
+// range.  f16: up to 65,504 * 1,024, in steps of 2^-34; a log-sum-exp over the
+// scale or a delta beyond that (scores of 6.7e7 before the scale) becomes NaN, as
+// does one that is no finite number, and so the gradients that it is part of.
 template <typename T> struct Split {
   static constexpr float k0 = 1.f, k1 = 1.f, k2 = 1.f, kMost = 1e38f;
 };
@@ -112,7 +114,7 @@ template <> struct Split<__half> {
 template <typename T>
 __device__ __forceinline__ uint4 split3(float v) {
   using S = Split<T>;
-  v = fminf(fmaxf(v, -S::kMost), S::kMost);
+  v = fabsf(v) <= S::kMost ? v : NAN;
   const float a = Cvt<T>::to_f(Cvt<T>::from_f(v / S::k0)), r = v - a * S::k0, b = Cvt<T>::to_f(Cvt<T>::from_f(r / S::k1));
   return make_uint4(pack2<T>(a, b), pack2<T>((r - b * S::k1) / S::k2, 0.f), 0u, 0u);
 }
@@ -143,8 +145,9 @@ __global__ void __launch_bounds__(256) k_da_stats(const DaBwd p, const __grid_co
   }
   if (lane < 4) {
     const float l = lane < 2 ? p.lse[(static_cast<int64_t>(lane) * p.heads + h) * p.nq + row] : 0.f;
+    // l = +inf: a row without keys, which none of its columns is used for
     p.split[(static_cast<int64_t>(lane) * p.heads + h) * p.np + r.aux + (row - r.q0)] =
-        split3<T>(lane < 2 ? -l / p.scale_log2 : lane == 2 ? -d1 : d1 - d2);
+        split3<T>(lane < 2 ? (l == INFINITY ? 0.f : -l / p.scale_log2) : lane == 2 ? -d1 : d1 - d2);
   }
 }
 
