@@ -292,6 +292,59 @@ def test_diff_attention_scales_and_gains(pkg, cuda):
     _close(got[2], ref, "dv", _half(HF))
 
 
+def _da_small_gradients(pkg, cuda, nq, nkv, gain, seed, heads=2, kv_heads=1, parts=((0, None),)):
+    """f16 gradients of one sequence where they, the weights or the score gradients are small or large: elementwise
+    as ever, and over the rows of each part the relative L2 bound of this file beside the absolute step of results
+    below the normal range (half of 2^-24 an element)."""
+    q, k, v, lam, dout = _da_inputs(cuda, nq, nkv, heads, kv_heads, HF, seed)
+    dout = (dout.float() * gain).to(HF)
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+    got = torch.autograd.grad(pkg.sparse_diff_attention(q, k, v, lam, [0, nq], [0, nkv]), leaves, dout)
+    ref = B.diff_attention(_f64(q), _f64(k), _f64(v), _f64(lam), [0, nq], [0, nkv], dout=_f64(dout), u=_half(HF))
+    for name, g in zip(("dq", "dk", "dv"), got):
+        err = np.abs(_f64(g) - ref[name])
+        assert np.isfinite(err).all() and (err <= ref[name + "_bound"] + 2.0 ** -25).all(), name
+        for first, step in parts if name == "dq" else ((0, None),):
+            e, r = err[first::step], ref[name][first::step]
+            most = (2 * _half(HF) + 2e-4) * np.linalg.norm(r) + 2.0 ** -25 * r.size ** 0.5
+            assert np.linalg.norm(e) <= most, (name, np.linalg.norm(e), most)
+
+
+@pytest.mark.parametrize("gain", [1.0, 2.0 ** -7, 2.0 ** -10, 2.0 ** -14])
+def test_diff_attention_f16_small_gradients(pkg, cuda, gain):
+    """dout as a mean over many values makes it, weights of 1 / 8192."""
+    _da_small_gradients(pkg, cuda, 256, 8192, gain, 60)
+
+
+def test_diff_attention_f16_small_weights(pkg, cuda):
+    """Weights of 5e-6, below f16's normal range: dv is made from them."""
+    _da_small_gradients(pkg, cuda, 64, 200_000, 64.0, 61, heads=1)
+
+
+def test_diff_attention_f16_large_gradients(pkg, cuda):
+    """dP - delta past 65,504, as under a loss scale, with gradients that fit."""
+    _da_small_gradients(pkg, cuda, 4, 8, 2.0 ** 13, 62)
+
+
+def test_diff_attention_f16_rows_of_other_size(pkg, cuda):
+    """Rows whose dout is 2^-10 of the others' keep their dq."""
+    gain = torch.ones(256, 1, 1, device=cuda)
+    gain[::2] = 2.0 ** -10
+    _da_small_gradients(pkg, cuda, 256, 8192, gain, 63, parts=((0, 2), (1, 2)))
+
+
+def test_diff_attention_f16_large_lam(pkg, cuda):
+    """lam far from 1 scales one map's score gradients and its part of the weights."""
+    for lam in (40.0, -0.01, 0.0):
+        q, k, v, _, dout = _da_inputs(cuda, 200, 300, 4, 2, HF, 64)
+        leaves = [t.requires_grad_() for t in (q, k, v)]
+        got = torch.autograd.grad(pkg.sparse_diff_attention(q, k, v, lam, [0, 200], [0, 300]), leaves, dout)
+        ref = B.diff_attention(_f64(q), _f64(k), _f64(v), np.full(4, lam), [0, 200], [0, 300], dout=_f64(dout),
+                               u=_half(HF))
+        for name, g in zip(("dq", "dk", "dv"), got):
+            _close(g, ref, name, _half(HF))
+
+
 def test_diff_attention_prefill_beside_single_tokens(pkg, cuda):
     """Sequences whose keys are cut into ranges beside some whose are not."""
     for dtype in (BF, HF):

@@ -37,6 +37,15 @@
 // products, which f32 operands would halve in rate at least: dq is off by 0.0026
 // relative in bf16 (2^-8 an element, averaged by the sum), 0.0017 in f32 with a
 // rounded result.  Scores, statistics and accumulators stay f32.
+// f16 has 2^-24 to 65,504 where weights of n keys are about 1 / n and score
+// gradients less, so there the operands are scaled by powers of two, taken out
+// of the f32 sums again.  With |dP - delta| <= 2 |dO_i| max_j |V_j| (O is a mean
+// of V rows), a query's dS in the dQ kernel get the factor that takes this bound
+// times max(1, |lam|) below 2^15; in the dK / dV kernel, whose rows sum over
+// queries, dS get one for the sequence and its key / value head, and P - lam P_2
+// one that takes 1 + |lam| there.  The factors of P are added to its exponent.
+// k_da_top takes the norms' maxima.  8,192 keys, dO of 2^-14: dq off by 0.059
+// relative without, as the rounding of its result alone (0.006) with the factors.
 // Few CTAs: the walk is cut into ranges whose f32 sums k_da_bwd_join adds in order.
 // Every mbarrier wait is bounded (SC_ETIMEOUT).
 #include "sc_diffattn_dev.cuh"
@@ -79,9 +88,12 @@ struct DaBwd {
   const float* lse;    // [2][heads][nq]
   const float* maps;   // [nq][heads][2][128]
   const void* dout;
-  float* st;           // [5][heads][np]: -lse_1, -lse_2, -delta_1, -delta_2, delta_1 - delta_2
+  float* st;           // [5][heads][np]: -lse_1, -lse_2, -delta_1, -delta_2, delta_1 - delta_2; f16: a sixth, the
+                       // exponent of the row's factor
   uint4* split;        // [4][heads][np] rows of eight values: -lse_m / c, -delta_1, delta_1 - delta_2 in three parts
   int64_t np;          // rows of st and split: sequences start at multiples of 4
+  const float* top;    // f16: [2][batch][kv_heads] largest |V_j|^2 and |dO_i|^2 (records: part0 = batch entry)
+  int batch;
   void *dq, *dk, *dv, *dlam;
   float* part;         // [splits][rows of X][heads of X][dX_1 dX_2 (dV)], when the walk is cut
   int64_t nx;          // rows of X in all
@@ -101,6 +113,8 @@ __device__ __forceinline__ unsigned long long mul_f2(unsigned long long a, unsig
   asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
   return d;
 }
+// Whether score gradients and weights are scaled into the type's range.
+template <typename T> constexpr bool kScaled = std::is_same_v<T, __half>;
 // A statistic v as three values of T, v = k0 a + k1 b + k2 c.  bf16 has f32's
 // range.  f16: up to 65,504 * 1,024, in steps of 2^-34; a log-sum-exp over the
 // scale or a delta beyond that (scores of 6.7e7 before the scale) becomes NaN, as
@@ -119,6 +133,54 @@ __device__ __forceinline__ uint4 split3(float v) {
   return make_uint4(pack2<T>(a, b), pack2<T>((r - b * S::k1) / S::k2, 0.f), 0u, 0u);
 }
 
+// Whole e with 2^e bound < 2^want (and no less than half of it); `none` where
+// bound is zero, infinite or NaN.
+__device__ __forceinline__ int pow2_to(float bound, int want, int none) {
+  if (!(bound > 0.f && bound < INFINITY)) return none;
+  return max(-100, min(100, want - (__float_as_int(bound) >> 23) + 126));
+}
+__device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) << 23); }
+
+template <typename T>
+__device__ __forceinline__ float4 load_f4(const T* p) {
+  const uint2 raw = *reinterpret_cast<const uint2*>(p);
+  const T* t = reinterpret_cast<const T*>(&raw);
+  return make_float4(Cvt<T>::to_f(t[0]), Cvt<T>::to_f(t[1]), Cvt<T>::to_f(t[2]), Cvt<T>::to_f(t[3]));
+}
+
+// Largest squared norm of the 128-wide rows of each sequence and key / value
+// head: top[sequence][group], zero before.  One CTA per (kTopRows rows, head),
+// records: item0 counts such blocks, aux = the sequence.  The maximum of the
+// bits of numbers that are not negative is theirs, NaN on top.
+constexpr int kTopRows = 64;
+template <typename T>
+__global__ void __launch_bounds__(256) k_da_top(const T* x, int64_t stride, int rep, int groups, float* top,
+                                                const __grid_constant__ SeqPlan plan) {
+  __shared__ int s[8];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const SeqRec& r = plan.at(plan.find(blockIdx.x));
+  const int64_t lo = r.q0 + static_cast<int64_t>(blockIdx.x - r.item0) * kTopRows;
+  const int64_t hi = min(lo + kTopRows, static_cast<int64_t>(r.q1));
+  float4 v[kTopRows / 8];  // every load ahead of the first use
+#pragma unroll
+  for (int k = 0; k < kTopRows / 8; ++k) {
+    const int64_t i = lo + warp + 8 * k;
+    v[k] = i < hi ? load_f4(x + i * stride + blockIdx.y * kDaDv + 4 * lane) : make_float4(0.f, 0.f, 0.f, 0.f);
+  }
+  int most = 0;
+#pragma unroll
+  for (int k = 0; k < kTopRows / 8; ++k) {
+    const float n = warp_add(fmaf(v[k].x, v[k].x, v[k].y * v[k].y) + fmaf(v[k].z, v[k].z, v[k].w * v[k].w));
+    most = max(most, __float_as_int(n) & 0x7fffffff);
+  }
+  if (lane == 0) s[warp] = most;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < 8; ++w) most = max(most, s[w]);
+    atomicMax(reinterpret_cast<int*>(top) + static_cast<int64_t>(r.aux) * groups + blockIdx.y / rep, most);
+  }
+}
+
 // Statistics of every (row, head), one warp each.  Records: aux = the
 // sequence's first row in st.
 template <typename T>
@@ -130,11 +192,16 @@ __global__ void __launch_bounds__(256) k_da_stats(const DaBwd p, const __grid_co
   const SeqRec& r = plan.at(plan.find(row));
   const float4 o1 = reinterpret_cast<const float4*>(p.maps + at * 2 * kDaDv)[lane];
   const float4 o2 = reinterpret_cast<const float4*>(p.maps + at * 2 * kDaDv + kDaDv)[lane];
-  const uint2 raw = reinterpret_cast<const uint2*>(static_cast<const T*>(p.dout) + at * kDaDv)[lane];
-  const T* g = reinterpret_cast<const T*>(&raw);
-  const float g0 = Cvt<T>::to_f(g[0]), g1 = Cvt<T>::to_f(g[1]), g2 = Cvt<T>::to_f(g[2]), g3 = Cvt<T>::to_f(g[3]);
-  const float d1 = warp_add(fmaf(g0, o1.x, g1 * o1.y) + fmaf(g2, o1.z, g3 * o1.w));
-  const float d2 = warp_add(fmaf(g0, o2.x, g1 * o2.y) + fmaf(g2, o2.z, g3 * o2.w));
+  const float4 g = load_f4(static_cast<const T*>(p.dout) + at * kDaDv + 4 * lane);
+  const float d1 = warp_add(fmaf(g.x, o1.x, g.y * o1.y) + fmaf(g.z, o1.z, g.w * o1.w));
+  const float d2 = warp_add(fmaf(g.x, o2.x, g.y * o2.y) + fmaf(g.z, o2.z, g.w * o2.w));
+  if constexpr (kScaled<T>) {
+    const float n = warp_add(fmaf(g.x, g.x, g.y * g.y) + fmaf(g.z, g.z, g.w * g.w));
+    const float v = p.top[static_cast<int64_t>(r.part0) * p.kv_heads + h / p.rep];
+    if (lane == 0)
+      p.st[(5ll * p.heads + h) * p.np + r.aux + (row - r.q0)] =
+          static_cast<float>(pow2_to(2.f * sqrtf(n * v) * fmaxf(1.f, fabsf(p.lam.get(h))), 15, 0));
+  }
   if (lane < 5) {
     const float l = lane < 2 ? p.lse[(static_cast<int64_t>(lane) * p.heads + h) * p.nq + row] : 0.f;
     const float v = lane < 2 ? -l : lane == 2 ? -d1 : lane == 3 ? -d2 : d1 - d2;
@@ -428,13 +495,33 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int hi = KV ? lq : (live ? key_limit(rec, x, p.causal) : y1);
     const int lo_max = __reduce_max_sync(0xffffffffu, lo), hi_min = __reduce_min_sync(0xffffffffu, hi);
     float nl[2] = {0.f, 0.f}, nd[2] = {0.f, 0.f};
-    if (!KV && live)
+    // factors out of the accumulators; where X are keys, into P (2^lift) and into dP - delta (fac)
+    float out_x = p.scale, out_v = 1.f, lift = 0.f, fac = 1.f;
+    if (!KV && live) {
+      const int64_t at = static_cast<int64_t>(blockIdx.y) * p.np + rec.aux + x, step = static_cast<int64_t>(p.heads) * p.np;
 #pragma unroll
       for (int m = 0; m < 2; ++m) {
-        const int64_t at = static_cast<int64_t>(blockIdx.y) * p.np + rec.aux + x;
-        nl[m] = p.st[m * static_cast<int64_t>(p.heads) * p.np + at];
-        nd[m] = p.st[(2 + m) * static_cast<int64_t>(p.heads) * p.np + at];
+        nl[m] = p.st[m * step + at];
+        nd[m] = p.st[(2 + m) * step + at];
       }
+      if constexpr (kScaled<T>) {
+        const float e = p.st[5 * step + at];
+        nl[0] += e;
+        nl[1] += e;
+        out_x *= pow2(-static_cast<int>(e));
+      }
+    }
+    if constexpr (KV && kScaled<T>) {
+      float most = 1.f;
+      for (int i = 0; i < (p.lam.count == 1 || !p.lam.p ? 1 : p.rep); ++i) most = fmaxf(most, fabsf(p.lam.get(g * p.rep + i)));
+      const float* top = p.top + static_cast<int64_t>(rec.part0) * p.kv_heads + g;
+      const int b = pow2_to(1.f + most, 15, 0);
+      const int f = pow2_to(2.f * sqrtf(top[0] * top[static_cast<int64_t>(p.batch) * p.kv_heads]) * most, 15 - b, -b);
+      lift = static_cast<float>(b);
+      fac = pow2(f);
+      out_v = pow2(-b);
+      out_x *= out_v * pow2(-f);
+    }
     bool ok = true;
     const unsigned long long sc2 = f2(p.scale_log2, p.scale_log2);
     // tile and head of the group's step, its place in the ring
@@ -471,7 +558,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int i = 0; i < kY; i += 2) {
           const unsigned long long x2 = f2(w[m][i], w[m][i + 1]);
           float a, b;
-          f2_split(KV ? mul_f2(x2, sc2) : fma_f2(x2, sc2, f2(nl[m], nl[m])), a, b);
+          f2_split(!KV             ? fma_f2(x2, sc2, f2(nl[m], nl[m]))
+                   : kScaled<T> ? fma_f2(x2, sc2, f2(lift, lift))
+                                : mul_f2(x2, sc2),
+                   a, b);
           w[m][i] = ex2_ftz(a);
           w[m][i + 1] = ex2_ftz(b);
         }
@@ -514,7 +604,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int e = 0; e < kY; e += 2) {
         // dP - delta_1 and dP - delta_2
         unsigned long long d1 = f2(dp[e], dp[e + 1]), d2;
-        if (KV) {
+        if (KV && kScaled<T>) {
+          d1 = mul_f2(d1, f2(fac, fac));
+          d2 = fma_f2(f2(diff[e], diff[e + 1]), f2(fac, fac), d1);
+        } else if (KV) {
           d2 = add_f2(d1, f2(diff[e], diff[e + 1]));
         } else {
           d2 = add_f2(d1, f2(nd[1], nd[1]));
@@ -566,7 +659,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (n > 0) tmem_ld32(lane_base + (part ? C::kV : C::kAcc) + 64u * grp + 32u * c, o);
         const int col = 64 * grp + 32 * c;
 #pragma unroll
-        for (int i = 0; i < 32; ++i) o[i] = ok ? o[i] * (part ? 1.f : p.scale) : 0.f;
+        for (int i = 0; i < 32; ++i) o[i] = ok ? o[i] * (part ? out_v : out_x) : 0.f;
         if (live && p.part) {
           float4* dst = reinterpret_cast<float4*>(p.part + (blockIdx.z * p.nx * xheads + at) * kWide + 128 * part + col);
 #pragma unroll
@@ -623,7 +716,7 @@ sc_status launch_bwd(Handle* h, const DaArgs& a, DaBwd p, const std::vector<int3
   std::vector<SeqRec> recs;
   for (int b = 0; b < a.batch; ++b)
     if (KV ? a.cu_kv[b + 1] > a.cu_kv[b] : a.cu_q[b + 1] > a.cu_q[b])
-      recs.push_back(SeqRec{a.cu_q[b], a.cu_q[b + 1], a.cu_kv[b], a.cu_kv[b + 1], 0, st_row[b]});
+      recs.push_back(SeqRec{a.cu_q[b], a.cu_q[b + 1], a.cu_kv[b], a.cu_kv[b + 1], 0, st_row[b], b});
   if (recs.empty()) return SC_OK;
   // the longest walks first: the tail of the launch is made of short CTAs
   std::stable_sort(recs.begin(), recs.end(), [](const SeqRec& x, const SeqRec& y) {
@@ -685,6 +778,28 @@ sc_status launch_bwd(Handle* h, const DaArgs& a, DaBwd p, const std::vector<int3
   return e == cudaSuccess ? SC_OK : cuda_error(h, e, "differential attention backward launch");
 }
 
+// top[sequence][group] of the rows of x (k_da_top), `heads` of them a token.
+template <typename T>
+sc_status launch_top(Handle* h, const void* x, int64_t stride, const int32_t* cu, int batch, int heads, int groups,
+                     float* top) {
+  std::vector<SeqRec> recs;
+  int64_t items = 0;
+  for (int b = 0; b < batch; ++b) {
+    if (cu[b + 1] == cu[b]) continue;
+    recs.push_back(SeqRec{cu[b], cu[b + 1], 0, 0, static_cast<int32_t>(items), b});
+    items += (cu[b + 1] - cu[b] + kTopRows - 1) / kTopRows;
+  }
+  if (recs.empty()) return SC_OK;
+  SeqPlan plan;
+  DevBuf table(h);
+  const sc_status st = make_plan(h, recs, &plan, &table.p);
+  if (st != SC_OK) return st;
+  ++h->launches;
+  k_da_top<T><<<dim3(static_cast<unsigned>(items), heads), 256, 0, h->stream>>>(static_cast<const T*>(x), stride,
+                                                                              heads / groups, groups, top, plan);
+  return SC_OK;
+}
+
 template <typename T>
 sc_status run_backward(Handle* h, const DaArgs& a) {
   const int64_t nq = a.cu_q[a.batch];
@@ -712,19 +827,30 @@ sc_status run_backward(Handle* h, const DaArgs& a) {
   for (int b = 0; b < a.batch; ++b) {
     st_row[b] = static_cast<int32_t>(rows);
     if (a.cu_q[b + 1] == a.cu_q[b]) continue;
-    recs.push_back(SeqRec{a.cu_q[b], a.cu_q[b + 1], 0, 0, a.cu_q[b], st_row[b]});
+    recs.push_back(SeqRec{a.cu_q[b], a.cu_q[b + 1], 0, 0, a.cu_q[b], st_row[b], b});
     rows += (a.cu_q[b + 1] - a.cu_q[b] + 3) / 4 * 4;
     if (rows > 0x7fffff00) return set_error(h, SC_EINVAL, "differential attention backward: too many rows");
   }
   p.np = rows + Cfg<true>::kY;  // a tile's copy may reach behind the last row
   const size_t per = static_cast<size_t>(a.heads) * p.np;
   DevBuf buf(h);
-  cudaError_t e = dev_alloc(h, &buf.p, per * (4 * sizeof(uint4) + 5 * sizeof(float)));
+  const size_t tops = kScaled<T> ? static_cast<size_t>(a.batch) * a.kv_heads : 0;
+  cudaError_t e = dev_alloc(h, &buf.p, per * (4 * sizeof(uint4) + (kScaled<T> ? 6 : 5) * sizeof(float)) +
+                                           2 * tops * sizeof(float));
   p.split = static_cast<uint4*>(buf.p);
   if (e != cudaSuccess) return cuda_error(h, e, "differential attention workspace");
   p.st = reinterpret_cast<float*>(p.split + 4 * per);
+  p.batch = a.batch;
   sc_status st = SC_OK;
-  if (nq > 0) {
+  if constexpr (kScaled<T>) {
+    float* top = p.st + 6 * per;
+    p.top = top;
+    e = cudaMemsetAsync(top, 0, 2 * tops * sizeof(float), h->stream);
+    if (e != cudaSuccess) return cuda_error(h, e, "differential attention workspace");
+    st = launch_top<T>(h, a.v, a.vs, a.cu_kv, a.batch, a.kv_heads, a.kv_heads, top);
+    if (st == SC_OK) st = launch_top<T>(h, a.dout, 128ll * a.heads, a.cu_q, a.batch, a.heads, a.kv_heads, top + tops);
+  }
+  if (st == SC_OK && nq > 0) {
     SeqPlan plan;
     DevBuf table(h);
     st = make_plan(h, recs, &plan, &table.p);
