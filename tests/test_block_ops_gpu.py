@@ -333,6 +333,24 @@ def test_diff_attention_f16_rows_of_other_size(pkg, cuda):
     _da_small_gradients(pkg, cuda, 256, 8192, gain, 63, parts=((0, 2), (1, 2)))
 
 
+@pytest.mark.parametrize("nq", [1, 150])
+def test_diff_attention_f16_weights_far_below_the_largest(pkg, cuda, nq):
+    """500 keys of weight 2^-25 to 2^-26 beside one of weight 1 whose values are zero: all of the output comes from
+    them.  A weight is off by at most 2^-32 of the row's largest (half a step of f16's smallest numbers, weights
+    written 2^7 times larger)."""
+    rng = np.random.default_rng(65)
+    q = torch.ones(nq, 2, 64, dtype=HF, device=cuda)
+    k = torch.from_numpy(rng.uniform(-1.14, -1.08, (500, 2, 1)).astype(np.float32)).to(cuda, HF).repeat(1, 1, 64)
+    k[37] = 1.1
+    v = torch.full((500, 1, 128), 1000.0, dtype=HF, device=cuda)
+    v[37] = 0
+    cu_q, cu_kv = [0, nq], [0, 500]
+    got = pkg.sparse_diff_attention(q, k, v, -1.0, cu_q, cu_kv)
+    ref = B.diff_attention(_f64(q), _f64(k), _f64(v), np.array([-1.0]), cu_q, cu_kv, u=_half(HF))
+    assert ref["out"].min() > 0.01
+    assert (np.abs(_f64(got) - ref["out"]) <= ref["out_bound"] + 2 * 2.0 ** -32 * 499 * 1000).all()
+
+
 def test_diff_attention_f16_large_lam(pkg, cuda):
     """lam far from 1 scales one map's score gradients and its part of the weights."""
     for lam in (40.0, -0.01, 0.0):

@@ -54,6 +54,10 @@ constexpr int kSmem = kOffBar + 256 + 1024;
 constexpr uint32_t kTmem = 512;            // S | P_1 | P_2 | O_1 | O_2
 constexpr uint32_t kColP = 128, kColO = 256;  // + 64 m, + 128 m
 constexpr float kRescale = 8.f;            // log2
+// f16 weights are written 2^7 times larger, between 2^7 and 2^15 where they are
+// largest: f16 has steps of 2^-24 at least, so unlifted it drops keys below 2^-25
+// of the row's largest weight, which 100,000 keys can make a hundredth of a row.
+template <typename T> constexpr float kLift = std::is_same_v<T, __half> ? 7.f : 0.f;
 
 struct DaFwd {
   LamRef lam;
@@ -278,8 +282,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int i = 16; i < kTile; i += 2) mv[(i >> 1) & 7] = max3(mv[(i >> 1) & 7], s[i / 64][i % 64], s[i / 64][i % 64 + 1]);
         const float top = fmaxf(fmaxf(fmaxf(mv[0], mv[1]), fmaxf(mv[2], mv[3])),
                                 fmaxf(fmaxf(mv[4], mv[5]), fmaxf(mv[6], mv[7]))) * p.scale_log2;
-        const bool move = top > mx + kRescale;  // true for the first visible key (mx = -inf)
-        const float m_new = move ? top : mx;
+        const bool move = top > mx + kLift<T> + kRescale;  // true for the first visible key (mx = -inf)
+        const float m_new = move ? top - kLift<T> : mx;
         const float alpha = move ? ex2_ftz(mx - m_new) : 1.f;
         // the product of this map's last step: O_m is complete and P_m is read
         if (j > 0) {
