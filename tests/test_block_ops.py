@@ -134,6 +134,18 @@ def test_group_norm_passes_dense_weights(pkg, monkeypatch, grad):
         np.testing.assert_array_equal(gb, b.numpy())
 
 
+def test_dual_tensors_take_part_in_autograd(pkg):
+    """They go to the autograd function, as tensors that require grad do (which refuses them: see the GPU tests)."""
+    from torch.autograd import forward_ad
+    wants, x = pkg.block_ops._wants_grad, torch.zeros(2, 2)
+    assert not wants(x, None, 0.5) and wants(x, torch.zeros(1, requires_grad=True), None)
+    with torch.no_grad():
+        assert not wants(torch.zeros(1, requires_grad=True))
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, torch.ones(2, 2))
+        assert not wants(x) and wants(None, dual)
+
+
 def test_diff_attention_refusals(pkg):
     h = torch.bfloat16
     q, k, v = torch.zeros(5, 8, 64, dtype=h), torch.zeros(7, 4, 64, dtype=h), torch.zeros(7, 2, 128, dtype=h)

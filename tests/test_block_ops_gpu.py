@@ -558,6 +558,25 @@ def test_diff_attention_past_32_bit_offsets(pkg, cuda):
 
 
 # ------------------------------------------------------------------- together
+def test_forward_mode_is_refused(pkg, cuda):
+    """No tangent is dropped: torch's own error names the missing rule."""
+    from torch.autograd import forward_ad
+    x, w, b, dy = _gn_inputs(cuda, 40, 64, FP, FP, 13)
+    q, k, v, lam, _ = _da_inputs(cuda, 40, 40, 2, 1, BF, 66)
+    with forward_ad.dual_level():
+        for call in (lambda: pkg.sparse_group_norm(forward_ad.make_dual(x, dy), 8, w, b),
+                     lambda: pkg.sparse_group_norm(x, 8, forward_ad.make_dual(w, b), b),
+                     lambda: pkg.sparse_diff_attention(forward_ad.make_dual(q, q.clone()), k, v, lam, [0, 40]),
+                     lambda: pkg.sparse_diff_attention(q, k, v, forward_ad.make_dual(lam, lam.clone()), [0, 40])):
+            with pytest.raises((RuntimeError, NotImplementedError)):
+                call()
+            with torch.no_grad(), pytest.raises((RuntimeError, NotImplementedError)):
+                call()
+        assert pkg.sparse_group_norm(x, 8, w, b).shape == x.shape
+    with pytest.raises((RuntimeError, NotImplementedError)):
+        torch.func.jvp(lambda t: pkg.sparse_group_norm(t, 8, w, b), (x,), (dy,))
+
+
 def _block(pkg, x, p, cu, heads, kv_heads):
     """Norm, fused projection, differential attention, projection, skip."""
     y = pkg.sparse_group_norm(x, 32, p["w"], p["b"], cu_seqlens=cu, silu=True)

@@ -8,7 +8,8 @@ be called from any thread and captured into a CUDA graph (pass the offsets as
 host values then), and give the same bits on every run.  Errors from the
 library surface as ``SparseConvError``.
 
-Both support ``torch.autograd`` (first derivatives).  A backward pass captured
+Both support ``torch.autograd`` (first derivatives in reverse mode; forward
+mode is refused).  A backward pass captured
 into a graph goes through torch's own rules: use ``torch.autograd.grad``, and
 let no eager graph of the same leaves live meanwhile.
 """
@@ -19,6 +20,7 @@ import math
 import operator
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib as L
 from .sparse_conv import _DTYPES, get_engine
@@ -57,6 +59,15 @@ def _p(t):
 def _dense(t):
     """An uninitialised dense tensor like ``t``."""
     return torch.empty_like(t, memory_format=torch.contiguous_format)
+
+
+def _wants_grad(*inputs):
+    """Whether autograd takes part: an input requires grad, or is dual.  A dual one goes to the autograd function too,
+    which has no forward-mode rule, so that torch says so instead of dropping the tangent."""
+    tensors = [t for t in inputs if isinstance(t, torch.Tensor)]
+    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+        return True
+    return forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
 def _overlap(a, b):
@@ -168,8 +179,7 @@ def sparse_group_norm(x, num_groups, weight=None, bias=None, eps=1e-5, cu_seqlen
     cu = _offsets([0, n] if cu_seqlens is None else cu_seqlens, n, "cu_seqlens")
     if not x.is_cuda:
         raise ValueError("sparse_group_norm runs on CUDA tensors only")
-    grad = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias))
-    if grad:
+    if _wants_grad(x, weight, bias):
         if out is not None:
             raise ValueError("out= takes no part in autograd: use it under torch.no_grad()")
         return _GroupNorm.apply(x, weight, bias, groups, eps, cu, bool(silu))
@@ -295,7 +305,7 @@ def sparse_diff_attention(q, k, v, lam, cu_seqlens_q, cu_seqlens_kv=None, scale=
     if not q.is_cuda:
         raise ValueError("sparse_diff_attention runs on CUDA tensors only")
     leaves = [t for t in (q, k, v, lam) if isinstance(t, torch.Tensor)]
-    if torch.is_grad_enabled() and any(t.requires_grad for t in leaves):
+    if _wants_grad(*leaves):
         if out is not None:
             raise ValueError("out= takes no part in autograd: use it under torch.no_grad()")
         return _DiffAttention.apply(q, k, v, lam, cu_q, cu_kv, scale, bool(causal))
