@@ -682,6 +682,37 @@ def test_from_several_threads(pkg, cuda):
     assert not bad
 
 
+def test_group_norm_from_two_handles(pkg, cuda):
+    """Calls of one kernel with more and with less shared memory at the same time, a handle per thread."""
+    import ctypes
+    import threading
+    x = torch.randn(2, 4096, device=cuda, dtype=BF)
+    cu = (ctypes.c_int32 * 2)(0, 2)
+    bad = []
+
+    def work(groups, stream):
+        engine, y = pkg.Engine(cuda), torch.empty_like(x)
+        with torch.cuda.stream(stream):
+            ref = pkg.sparse_group_norm(x, groups)
+            try:
+                for _ in range(4000):
+                    engine.call("sc_group_norm", x.data_ptr(), 4096, None, None, y.data_ptr(), None, cu, 1, 4096,
+                                groups, 1e-5, 0, pkg._lib.SC_BF16, pkg._lib.SC_BF16)
+                stream.synchronize()
+                if not torch.equal(y, ref):
+                    bad.append("values")
+            except Exception as e:  # noqa: BLE001
+                bad.append(e)
+        engine.close()
+    torch.cuda.synchronize()
+    ts = [threading.Thread(target=work, args=(g, torch.cuda.Stream(cuda))) for g in (4096, 2048, 4096, 2048)]
+    for t in ts:
+        t.start()
+    for t in ts:
+        t.join()
+    assert not bad, bad
+
+
 def test_captured_and_replayed(pkg, cuda):
     """Forward and backward of the block in a CUDA graph, two graphs replayed
     in turn with new inputs, against eager calls."""

@@ -782,6 +782,8 @@ bool gn_ring(const GnParams& p) {
   return V * sizeof(T) == 16 && p.xs == p.c && nvec <= kGnThreads && p.chunk >= 8 * (kGnThreads / nvec);
 }
 
+// The limit belongs to the kernel, not to the handle: always the largest that a
+// launch may need, so that calls of other threads do not lower it in between.
 template <typename... P>
 cudaError_t gn_allow_smem(void (*kernel)(P...), size_t bytes) {
   return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
@@ -790,6 +792,7 @@ cudaError_t gn_allow_smem(void (*kernel)(P...), size_t bytes) {
 // Sequences up to this many bytes per CTA of a cluster of eight take one kernel.
 constexpr int64_t kGnClusterBytes = 128 * 1024;
 constexpr int kGnClusterMax = 8;
+constexpr size_t kGnClusterSmem = 32 * 1024 + 4 * sizeof(float) * 4096;  // sums, then four floats a group
 
 template <typename T, int V, int GS>
 sc_status gn_forward_v(Handle* h, GnParams p, const int32_t* cu, int batch) {
@@ -809,8 +812,8 @@ sc_status gn_forward_v(Handle* h, GnParams p, const int32_t* cu, int batch) {
     // a rank for every eight rows of a row lane
     int ranks = 1;
     while (ranks < kGnClusterMax && longest > 8ll * ty * ranks) ranks *= 2;
-    const size_t smem = gn_sum_smem(p.c, p.c / V) + sizeof(float) * 4 * p.groups;  // at most 96 KB
-    e = smem > 48 * 1024 ? gn_allow_smem(k_gn_cluster<T, V, GS>, smem) : cudaSuccess;
+    const size_t smem = gn_sum_smem(p.c, p.c / V) + sizeof(float) * 4 * p.groups;
+    e = smem > 48 * 1024 ? gn_allow_smem(k_gn_cluster<T, V, GS>, kGnClusterSmem) : cudaSuccess;
     if (e == cudaSuccess)
       e = launch_ex(h, k_gn_cluster<T, V, GS>, static_cast<int>(recs.size()) * ranks, smem, ranks, p, call.plan, ranks);
   } else {
