@@ -146,6 +146,33 @@ def test_dual_tensors_take_part_in_autograd(pkg):
         assert not wants(x) and wants(None, dual)
 
 
+def test_engine_synchronizes_the_device_once_operators_ran(pkg, monkeypatch):
+    """The operators' handle is read after all streams, on the caller's stream; an engine that ran none waits for its
+    own stream alone, as before."""
+    import threading
+    done = []
+
+    class Library:
+        def __getattr__(self, name):
+            return lambda *args: done.append((name, *args)) or 0
+    engine = object.__new__(pkg.Engine)
+    engine.lib, engine.handle, engine._op_handle = Library(), None, "ops"
+    engine.device, engine._op_lock, engine._op_used = torch.device("cuda", 0), threading.Lock(), False
+    current = ["a"]
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda index: current[0], raising=False)
+    monkeypatch.setattr(torch.cuda, "synchronize", lambda device: done.append(("device", device)))
+    engine.synchronize()
+    assert done == [("sc_synchronize", None)]
+    engine.call("sc_group_norm", 1)
+    current[0] = "b"
+    engine.call("sc_group_norm", 2)
+    current[0] = "c"
+    done.clear()
+    engine.synchronize()
+    assert done == [("sc_synchronize", None), ("device", engine.device), ("sc_set_stream", "ops", "c"),
+                    ("sc_synchronize", "ops")]
+
+
 def test_diff_attention_refusals(pkg):
     h = torch.bfloat16
     q, k, v = torch.zeros(5, 8, 64, dtype=h), torch.zeros(7, 4, 64, dtype=h), torch.zeros(7, 2, 128, dtype=h)

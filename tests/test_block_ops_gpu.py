@@ -656,6 +656,24 @@ def test_repeatable_and_on_other_streams(pkg, cuda):
     pkg.get_engine(cuda).synchronize()
 
 
+def test_synchronize_waits_for_every_stream(pkg, cuda):
+    """Work that was called for on other streams than the last one, and in a replayed graph, is over after it."""
+    engine, x = pkg.get_engine(cuda), torch.randn(300, 64, device=cuda)
+    side, graph = torch.cuda.Stream(cuda), torch.cuda.CUDAGraph()
+    pkg.sparse_group_norm(x, 8)
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        pkg.sparse_group_norm(x, 8)
+    for replay in (False, True):
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(200_000_000)  # about 0.1 s
+            graph.replay() if replay else pkg.sparse_group_norm(x, 8)
+        pkg.sparse_group_norm(x, 8)
+        assert not side.query()
+        engine.synchronize()
+        assert side.query()
+
+
 def test_from_several_threads(pkg, cuda):
     import threading
     x, p, dy = _block_inputs(cuda, 500, 128, 4, 2, 42)

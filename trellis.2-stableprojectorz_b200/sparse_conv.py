@@ -64,6 +64,7 @@ class Engine:
         # A second handle for the operators whose backward pass autograd runs
         # on its own threads: its stream is bound and its calls made under a lock.
         self._op_lock = threading.Lock()
+        self._op_used = False
         oh = ctypes.c_void_p()
         st = self.lib.sc_create(ctypes.byref(oh), ctypes.byref(cfg))
         if st != L.SC_OK:
@@ -81,6 +82,7 @@ class Engine:
     def call(self, name, *args):
         """One library call on torch's current stream of this device, safe from any thread."""
         with self._op_lock:
+            self._op_used = True
             self.lib.sc_set_stream(self._op_handle, torch._C._cuda_getCurrentRawStream(self.device.index))
             st = getattr(self.lib, name)(self._op_handle, *args)
             if st != L.SC_OK:
@@ -95,9 +97,15 @@ class Engine:
         return int(self.lib.sc_launch_count(self.handle)) + int(self.lib.sc_launch_count(self._op_handle))
 
     def synchronize(self):
+        """Waits for the work of this engine and raises what its kernels reported."""
         self.check(self.lib.sc_synchronize(self.handle), "synchronize")
         with self._op_lock:
-            L.check(self.lib.sc_synchronize(self._op_handle), self._op_handle, "synchronize")
+            if self._op_used:
+                # call() ran on any number of streams, and graphs may replay what it captured: all of the
+                # device's work ends before the status is read, on a stream that is there
+                torch.cuda.synchronize(self.device)
+                self.lib.sc_set_stream(self._op_handle, torch._C._cuda_getCurrentRawStream(self.device.index))
+                L.check(self.lib.sc_synchronize(self._op_handle), self._op_handle, "synchronize")
 
     def close(self):
         for name in ("handle", "_op_handle"):
