@@ -558,6 +558,27 @@ def test_diff_attention_past_32_bit_offsets(pkg, cuda):
 
 
 # ------------------------------------------------------------------- together
+def test_out_is_known_to_autograd(pkg, cuda):
+    """A tensor that a backward pass saved may not be overwritten unnoticed; one that requires grad is no out."""
+    x, w, b, dy = _gn_inputs(cuda, 40, 64, BF, BF, 14)
+    q, k, v, _, _ = _da_inputs(cuda, 40, 40, 1, 1, BF, 67)
+    for write in (lambda t: pkg.sparse_group_norm(t, 8, w, b, out=t),
+                  lambda t: pkg.sparse_diff_attention(q[:20], k, v, 0.5, [0, 20], [0, 40], out=t.view(20, 1, 128))):
+        t, scale = x.clone(), torch.ones((), device=cuda, dtype=BF, requires_grad=True)
+        loss = (t * scale).sum()
+        write(t)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            loss.backward()
+    out = torch.empty_like(x).requires_grad_()
+    with pytest.raises(ValueError, match="requires grad"):
+        pkg.sparse_group_norm(x, 8, w, b, out=out)
+    with torch.no_grad():
+        assert pkg.sparse_group_norm(x, 8, w, b, out=out) is out
+    with torch.inference_mode():
+        t = x.clone()
+        assert torch.equal(pkg.sparse_group_norm(t, 8, w, b, out=t), out)
+
+
 def test_forward_mode_is_refused(pkg, cuda):
     """No tangent is dropped: torch's own error names the missing rule."""
     from torch.autograd import forward_ad

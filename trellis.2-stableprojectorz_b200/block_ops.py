@@ -86,6 +86,14 @@ def _check_out(out, shape, like):
     if tuple(out.shape) != tuple(shape) or out.dtype != like.dtype or out.device != like.device or \
             not out.is_contiguous():
         raise ValueError(f"out must be a contiguous {tuple(shape)} {like.dtype} tensor on {like.device}")
+    if out.requires_grad and torch.is_grad_enabled():
+        raise ValueError("out= takes no part in autograd: out requires grad")
+
+
+def _written(out):
+    """``out`` after the library wrote it: autograd refuses a backward pass that saved what it held before."""
+    torch.autograd.graph.increment_version(out)
+    return out
 
 
 def _rows_view(x):
@@ -188,7 +196,8 @@ def sparse_group_norm(x, num_groups, weight=None, bias=None, eps=1e-5, cu_seqlen
         same = out.data_ptr() == x.data_ptr() and x.is_contiguous()
         if (_overlap(out, x) and not same) or _overlap(out, weight) or _overlap(out, bias):
             raise ValueError("out overlaps an input (only a contiguous x itself may be written in place)")
-    return _gn_forward(x, groups, weight, bias, eps, cu, silu, out, False)[0]
+    y, _ = _gn_forward(x, groups, weight, bias, eps, cu, silu, out, False)
+    return y if out is None else _written(out)
 
 
 # ------------------------------------------------------ differential attention
@@ -309,7 +318,8 @@ def sparse_diff_attention(q, k, v, lam, cu_seqlens_q, cu_seqlens_kv=None, scale=
         if out is not None:
             raise ValueError("out= takes no part in autograd: use it under torch.no_grad()")
         return _DiffAttention.apply(q, k, v, lam, cu_q, cu_kv, scale, bool(causal))
-    if out is None:
+    given = out is not None
+    if not given:
         out = torch.empty((q.shape[0], heads, 128), dtype=q.dtype, device=q.device)
     else:
         _check_out(out, (q.shape[0], heads, 128), q)
@@ -317,4 +327,4 @@ def sparse_diff_attention(q, k, v, lam, cu_seqlens_q, cu_seqlens_kv=None, scale=
             raise ValueError("out must be 16-byte aligned and overlap no input")
     a, hold = _da_args(q, k, v, lam, cu_q, cu_kv, scale, causal, out=out)
     get_engine(q.device).call("sc_diff_attention", ctypes.byref(a))
-    return out
+    return _written(out) if given else out
