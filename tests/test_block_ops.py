@@ -171,6 +171,9 @@ def test_engine_synchronizes_the_device_once_operators_ran(pkg, monkeypatch):
     engine.synchronize()
     assert done == [("sc_synchronize", None), ("device", engine.device), ("sc_set_stream", "ops", "c"),
                     ("sc_synchronize", "ops")]
+    done.clear()
+    engine.close()  # not on a stream that its caller may have destroyed
+    assert done == [("sc_set_stream", "ops", None), ("sc_destroy", "ops")] and engine._op_handle is None
 
 
 def test_diff_attention_refusals(pkg):

@@ -108,6 +108,9 @@ class Engine:
                 L.check(self.lib.sc_synchronize(self._op_handle), self._op_handle, "synchronize")
 
     def close(self):
+        if getattr(self, "_op_handle", None):
+            # the last caller's stream may be gone; freeing the handle's memory waits for the device
+            self.lib.sc_set_stream(self._op_handle, None)
         for name in ("handle", "_op_handle"):
             if getattr(self, name, None):
                 self.lib.sc_destroy(getattr(self, name))
