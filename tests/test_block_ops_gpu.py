@@ -89,6 +89,43 @@ def test_group_norm_large(pkg, cuda):
     _gn_check(pkg, cuda, [40000, 123, 60000], 64, 16, BF, FP, silu=True, seed=6)
 
 
+@pytest.mark.parametrize("dtype,wdtype,lens,c,groups,silu", [
+    (BF, FP, [20011, 1, 0, 30007, 123, 15003], 256, 32, True),  # vectors of one group
+    (BF, BF, [105003], 96, 3, True), (BF, BF, [60001, 45007], 96, 8, False),  # 504 of 512 threads have a column
+    (HF, HF, [50021, 30011], 128, 32, True), (HF, FP, [80033], 128, 4, False),
+    (FP, FP, [80033], 64, 16, True), (FP, FP, [50021, 2, 30011], 64, 32, True), (FP, FP, [80033], 64, 64, False),
+    (BF, FP, [3001, 1999], 2048, 16, True), (BF, BF, [2000, 707], 4096, 32, True)])
+def test_group_norm_through_the_ring(pkg, cuda, dtype, wdtype, lens, c, groups, silu):
+    """Rows through the ring of bulk copies, forward and backward, last blocks short: all rows and gradients."""
+    vectors = c * torch.finfo(dtype).bits // 128
+    slots = 2 * torch.cuda.get_device_properties(cuda).multi_processor_count
+    assert sum(lens) >= slots * 8 * (512 // vectors)  # chunks of eight rows a thread at least
+    _gn_check(pkg, cuda, lens, c, groups, dtype, wdtype, silu, seed=70)
+
+
+@pytest.mark.parametrize("dtype,c,groups,wide", [(BF, 64, 16, 16), (BF, 72, 8, 8), (HF, 66, 11, 3), (FP, 64, 32, 4)])
+def test_group_norm_long_rows_without_the_ring(pkg, cuda, dtype, c, groups, wide):
+    """Rows apart, as in a slice of a fused buffer, also of no whole 16-byte words: several chunks of many rows."""
+    cu = _cu([70001, 30, 29007])
+    x, w, b, dy = _gn_inputs(cuda, cu[-1], c, dtype, FP, 71)
+    x = torch.cat((dy[:, :wide], x), 1)[:, wide:].requires_grad_()
+    w.requires_grad_(), b.requires_grad_()
+    y = pkg.sparse_group_norm(x, groups, w, b, cu_seqlens=cu, silu=True)
+    got = (y, *torch.autograd.grad(y, (x, w, b), dy))
+    args = (groups, _f64(w), _f64(b), 1e-5, cu, True)
+    ref = (B.group_norm(_f64(x), *args), *B.group_norm_backward(_f64(x), _f64(dy), *args))
+    for g, r, t in zip(got, ref, (dtype, dtype, FP, FP)):
+        assert _rel(_f64(g), r) < (_half(t) if t != FP else 0) + 1e-5, (t, _rel(_f64(g), r))
+
+
+def test_group_norm_through_the_ring_in_place(pkg, cuda):
+    for dtype, c in ((BF, 256), (FP, 64)):
+        x, w, b, _ = _gn_inputs(cuda, 80033, c, dtype, FP, 72)
+        ref = pkg.sparse_group_norm(x, 16, w, b, silu=True, cu_seqlens=[0, 50001, 80033])
+        assert pkg.sparse_group_norm(x, 16, w, b, silu=True, cu_seqlens=[0, 50001, 80033], out=x) is x
+        assert torch.equal(x, ref)
+
+
 def test_group_norm_without_weights(pkg, oracle, cuda):
     x, _, b, dy = _gn_inputs(cuda, 400, 48, FP, FP, 7)
     y = pkg.sparse_group_norm(x, 6)
