@@ -581,6 +581,51 @@ def test_diff_attention_without_a_softmax(pkg, cuda, dtype):
             q = q.detach()
 
 
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("nq,nkv", [(0, 70), (70, 0), (0, 0)])
+def test_diff_attention_of_nothing(pkg, cuda, dtype, nq, nkv):
+    """No queries, or no keys, in the whole call: zeros, and gradients of zero."""
+    q, k, v, lam, dout = _da_inputs(cuda, nq, nkv, 4, 2, dtype, 53)
+    leaves = [t.requires_grad_() for t in (q, k, v, lam)]
+    out = pkg.sparse_diff_attention(*leaves, [0, 0, nq], [0, nkv, nkv], causal=True)
+    assert out.shape == (nq, 4, 128) and torch.count_nonzero(out) == 0
+    for g, t in zip(torch.autograd.grad(out, leaves, dout), leaves):
+        assert g.shape == t.shape and torch.count_nonzero(g) == 0
+
+
+@pytest.mark.parametrize("heads,kv_heads", [(129, 1), (256, 2), (128, 1)])
+def test_diff_attention_more_heads_than_a_tile_has_rows(pkg, cuda, heads, kv_heads):
+    _da_check(pkg, cuda, [3, 1, 140], [200, 70, 150], heads, kv_heads, BF, True, seed=54)
+    _da_check(pkg, cuda, [2], [700], heads, kv_heads, HF, False, seed=55, train=False)
+
+
+def test_diff_attention_f16_captured_and_repeated(pkg, cuda):
+    """f16 gradients (their factors come from maxima over the call) repeat bit for bit, also from a graph."""
+    cu = [0, 40, 41, 300]
+    q, k, v, lam, dout = _da_inputs(cuda, 300, 300, 4, 2, HF, 56)
+    leaves = [t.requires_grad_() for t in (q, k, v, lam)]
+
+    def run():
+        out = pkg.sparse_diff_attention(*leaves, cu, causal=True)
+        return [out.detach(), *torch.autograd.grad(out, leaves, dout)]
+    s = torch.cuda.Stream(cuda)
+    s.wait_stream(torch.cuda.current_stream(cuda))
+    with torch.cuda.stream(s):
+        run()
+    torch.cuda.current_stream(cuda).wait_stream(s)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = run()
+    for size in (1.0, 2.0 ** -12, 2.0 ** 8):
+        with torch.no_grad():
+            q.copy_(torch.randn_like(q))
+            dout.copy_(size * torch.randn_like(dout))
+        g.replay()
+        held = [t.clone() for t in got]
+        for _ in range(3):
+            assert all(torch.equal(a, b) for a, b in zip(held, run()))
+
+
 def test_diff_attention_past_32_bit_offsets(pkg, cuda):
     """A cache whose last sequence lies past 2^31 elements of k and v."""
     n, hk = 2_150_000, 8
