@@ -639,6 +639,48 @@ def test_diff_attention_past_32_bit_offsets(pkg, cuda):
     assert torch.count_nonzero(out[0]) == 0  # values of zero
 
 
+def test_refusals_of_the_c_calls(pkg, cuda):
+    """What the entry points refuse before any launch, with their reason; the handle stays usable."""
+    import ctypes
+    L, engine = pkg._lib, pkg.get_engine(cuda)
+    x = torch.randn(8, 64, device=cuda)
+    y, stats = torch.empty_like(x), torch.empty(16, device=cuda)
+    cu = lambda *a: (ctypes.c_int32 * len(a))(*a)  # noqa: E731
+
+    def refused(match, name, *args):
+        with pytest.raises(pkg.SparseConvError, match=match):
+            engine.call(name, *args)
+    gn = lambda x=x.data_ptr(), xs=64, y=y.data_ptr(), cu=cu(0, 8), batch=1, c=64, g=8, eps=1e-5, t=0, wt=0: (  # noqa: E731
+        x, xs, None, None, y, None, cu, batch, c, g, eps, 0, t, wt)
+    for match, bad in (("dtype", {"t": 9}), ("weight and bias", {"t": 0, "wt": 1}), ("channels", {"c": 4097, "g": 1}),
+                       ("channels", {"g": 7}), ("batch", {"batch": 0}), ("cu_seqlens", {"cu": None}),
+                       ("non-decreasing", {"cu": cu(0, 9, 8), "batch": 2}), ("start at 0", {"cu": cu(1, 8)}),
+                       ("x missing", {"x": None}), ("x_stride", {"xs": 63}), ("misaligned", {"x": x.data_ptr() + 2}),
+                       ("eps", {"eps": 0.0}), ("y missing", {"y": None})):
+        refused(match, "sc_group_norm", *gn(**bad))
+    refused("dy or stats", "sc_group_norm_backward", x.data_ptr(), 64, None, None, None, stats.data_ptr(), y.data_ptr(),
+            None, None, cu(0, 8), 1, 64, 8, 0, 0, 0)
+    q, k, v, lam, _ = _da_inputs(cuda, 8, 8, 2, 1, BF, 57)
+    out, offs = torch.empty(8, 2, 128, device=cuda, dtype=BF), cu(0, 8)
+    good = dict(q=q.data_ptr(), k=k.data_ptr(), v=v.data_ptr(), lam=lam.data_ptr(), q_stride=256, k_stride=128,
+                v_stride=128, cu_seqlens_q=ctypes.addressof(offs), cu_seqlens_kv=ctypes.addressof(offs), batch=1,
+                heads=2, kv_heads=1, lam_count=2, scale=0.125, dtype=L.SC_BF16, lam_dtype=L.SC_F32, out=out.data_ptr())
+    for match, bad in (("bf16 or f16", {"dtype": L.SC_F32}), ("heads", {"heads": 3, "kv_heads": 2}),
+                       ("heads", {"heads": 40000}), ("scale", {"scale": 0.0}), ("scale", {"scale": float("nan")}),
+                       ("lam_count", {"lam_count": 3}), ("lam must", {"lam_dtype": L.SC_F16}),
+                       ("q missing", {"q": None}), ("q missing", {"q": q.data_ptr() + 2}),
+                       ("q missing", {"q_stride": 260}), ("k or v", {"k_stride": 120}), ("k or v", {"v": None}),
+                       ("out missing", {"out": None}), ("go together", {"lse": stats.data_ptr()})):
+        refused(match, "sc_diff_attention", ctypes.byref(L.ScDiffAttentionArgs(**{**good, **bad})))
+    refused("backward needs", "sc_diff_attention_backward",
+            ctypes.byref(L.ScDiffAttentionArgs(**{**good, "dq": q.data_ptr()})))
+    refused("null arguments", "sc_diff_attention", None)
+    engine.call("sc_diff_attention", ctypes.byref(L.ScDiffAttentionArgs(**good)))
+    assert torch.equal(out, pkg.sparse_diff_attention(q, k, v, lam, [0, 8]))
+    engine.call("sc_group_norm", *gn())
+    assert torch.equal(y, pkg.sparse_group_norm(x, 8))
+
+
 # ------------------------------------------------------------------- together
 def test_out_is_known_to_autograd(pkg, cuda):
     """A tensor that a backward pass saved may not be overwritten unnoticed; one that requires grad is no out."""

@@ -256,10 +256,10 @@ sc_status sc_synchronize(sc_handle* h) {
     cudaMemsetAsync(H->derr, 0, sizeof(int), H->stream);
     cudaStreamSynchronize(H->stream);
     return sc::set_error(H, static_cast<sc_status>(err),
-                         err == SC_ETIMEOUT ? "device wait limit expired in a conv kernel"
+                         err == SC_ETIMEOUT ? "device wait limit expired in a kernel"
                          : err == SC_EINVAL ? "a kernel rejected an argument (halo push destination out of range or "
                                               "not 16-byte aligned)"
-                                            : "conv kernel error");
+                                            : "kernel error");
   }
   return SC_OK;
 }
@@ -649,13 +649,14 @@ sc_status sc_group_norm(sc_handle* h, const void* x, int64_t x_stride, const voi
                         float eps, int32_t apply_silu, sc_dtype dtype, sc_dtype wdtype) {
   if (!h) return SC_EINVAL;
   Handle* H = &h->impl;
-  const sc_status st = gn_check(H, x, x_stride, weight, bias, cu_seqlens, batch, channels, groups, dtype, wdtype);
-  if (st != SC_OK) return st;
-  if (!(eps > 0.f) || !(eps <= 3.0e38f)) return sc::set_error(H, SC_EINVAL, "group norm: eps must be positive and finite");
-  if (cu_seqlens[batch] == 0) return SC_OK;
-  if (!y || !sc::aligned(y, dtype_bytes(dtype)) || !sc::aligned(stats, 4))
-    return sc::set_error(H, SC_EINVAL, "group norm: y missing, or a misaligned pointer");
   return guarded(H, [&] {
+    const sc_status st = gn_check(H, x, x_stride, weight, bias, cu_seqlens, batch, channels, groups, dtype, wdtype);
+    if (st != SC_OK) return st;
+    if (!(eps > 0.f) || !(eps <= 3.0e38f))
+      return sc::set_error(H, SC_EINVAL, "group norm: eps must be positive and finite");
+    if (cu_seqlens[batch] == 0) return SC_OK;
+    if (!y || !sc::aligned(y, dtype_bytes(dtype)) || !sc::aligned(stats, 4))
+      return sc::set_error(H, SC_EINVAL, "group norm: y missing, or a misaligned pointer");
     sc::DeviceGuard g(H->device);
     return sc::group_norm(H, x, x_stride, weight, bias, y, stats, cu_seqlens, batch, channels, groups, eps,
                           apply_silu ? 1 : 0, dtype, wdtype);
@@ -668,24 +669,24 @@ sc_status sc_group_norm_backward(sc_handle* h, const void* x, int64_t x_stride, 
                                  int32_t apply_silu, sc_dtype dtype, sc_dtype wdtype) {
   if (!h) return SC_EINVAL;
   Handle* H = &h->impl;
-  const sc_status st = gn_check(H, x, x_stride, weight, bias, cu_seqlens, batch, channels, groups, dtype, wdtype);
-  if (st != SC_OK) return st;
-  if (!dx && !dweight && !dbias) return SC_OK;
-  if (!sc::aligned(dx, dtype_bytes(dtype)) || !sc::aligned(dweight, dtype_bytes(wdtype)) ||
-      !sc::aligned(dbias, dtype_bytes(wdtype)))
-    return sc::set_error(H, SC_EINVAL, "group norm: misaligned pointer");
-  sc::DeviceGuard g(H->device);
-  if (cu_seqlens[batch] == 0) {  // sums over nothing
-    for (void* p : {dweight, dbias})
-      if (p) {
-        const cudaError_t e = cudaMemsetAsync(p, 0, dtype_bytes(wdtype) * channels, H->stream);
-        if (e != cudaSuccess) return sc::cuda_error(H, e, "group norm: zero gradient");
-      }
-    return SC_OK;
-  }
-  if (!dy || !stats || !sc::aligned(dy, dtype_bytes(dtype)) || !sc::aligned(stats, 4))
-    return sc::set_error(H, SC_EINVAL, "group norm: dy or stats missing, or misaligned");
   return guarded(H, [&] {
+    const sc_status st = gn_check(H, x, x_stride, weight, bias, cu_seqlens, batch, channels, groups, dtype, wdtype);
+    if (st != SC_OK) return st;
+    if (!dx && !dweight && !dbias) return SC_OK;
+    if (!sc::aligned(dx, dtype_bytes(dtype)) || !sc::aligned(dweight, dtype_bytes(wdtype)) ||
+        !sc::aligned(dbias, dtype_bytes(wdtype)))
+      return sc::set_error(H, SC_EINVAL, "group norm: misaligned pointer");
+    sc::DeviceGuard g(H->device);
+    if (cu_seqlens[batch] == 0) {  // sums over nothing
+      for (void* p : {dweight, dbias})
+        if (p) {
+          const cudaError_t e = cudaMemsetAsync(p, 0, dtype_bytes(wdtype) * channels, H->stream);
+          if (e != cudaSuccess) return sc::cuda_error(H, e, "group norm: zero gradient");
+        }
+      return SC_OK;
+    }
+    if (!dy || !stats || !sc::aligned(dy, dtype_bytes(dtype)) || !sc::aligned(stats, 4))
+      return sc::set_error(H, SC_EINVAL, "group norm: dy or stats missing, or misaligned");
     return sc::group_norm_backward(H, x, x_stride, dy, weight, bias, stats, dx, dweight, dbias, cu_seqlens, batch,
                                    channels, groups, apply_silu ? 1 : 0, dtype, wdtype);
   });
@@ -694,8 +695,8 @@ sc_status sc_group_norm_backward(sc_handle* h, const void* x, int64_t x_stride, 
 sc_status sc_diff_attention(sc_handle* h, const sc_diff_attention_args* args) {
   if (!h) return SC_EINVAL;
   Handle* H = &h->impl;
-  if (!args) return sc::set_error(H, SC_EINVAL, "differential attention: null arguments");
   return guarded(H, [&] {
+    if (!args) return sc::set_error(H, SC_EINVAL, "differential attention: null arguments");
     sc::DaArgs a;
     const sc_status st = da_args(H, args, false, &a);
     if (st != SC_OK) return st;
@@ -708,8 +709,8 @@ sc_status sc_diff_attention(sc_handle* h, const sc_diff_attention_args* args) {
 sc_status sc_diff_attention_backward(sc_handle* h, const sc_diff_attention_args* args) {
   if (!h) return SC_EINVAL;
   Handle* H = &h->impl;
-  if (!args) return sc::set_error(H, SC_EINVAL, "differential attention: null arguments");
   return guarded(H, [&] {
+    if (!args) return sc::set_error(H, SC_EINVAL, "differential attention: null arguments");
     sc::DaArgs a;
     const sc_status st = da_args(H, args, true, &a);
     if (st != SC_OK) return st;
