@@ -277,9 +277,8 @@ SC_API sc_status sc_attention_varlen(sc_handle* h, const void* q, const void* k,
 SC_API sc_status sc_layernorm_silu(sc_handle* h, void* x, int64_t n, int32_t c, sc_dtype dtype, int32_t apply_silu,
                             float eps);
 
-/* Group norm over sparse sequences, channels last (the norm of the sparse
- * ResBlocks and attention blocks of the TRELLIS family; no counterpart in the
- * TS port, whose blocks use src/dense/ops/layer_norm.ts:28-60).  x is
+/* Group norm over sparse sequences, channels last (no counterpart in the TS
+ * port, whose blocks use the row norm of src/dense/ops/layer_norm.ts:28-60).  x is
  * [cu_seqlens[batch], channels] with x_stride elements between rows; every
  * (sequence, group) is normalised with the mean and the biased variance of its
  * rows x (channels / groups) values, then times weight plus bias ([channels] in
@@ -309,14 +308,16 @@ SC_API sc_status sc_group_norm_backward(sc_handle* h, const void* x, int64_t x_s
  *                - lam_h softmax_j(scale q[i, 2h+1] . k[j, 2g+1])) v[j, g]
  * over the sequence's key rows j; with causal, query i of the sequence sees
  * keys j <= i + len_kv - len_q.  A row that sees no key is zero (and passes no
- * gradient).  Two maps beside the one of sc_attention_varlen; q [Nq, 2 heads,
+ * gradient); NaN and +inf scores, and rows whose scores are all -inf, give NaN.
+ * Two maps beside the one of sc_attention_varlen; q [Nq, 2 heads,
  * 64], k [Nkv, 2 kv_heads, 64], v [Nkv, kv_heads, 128], out [Nq, heads, 128] in
  * dtype (bf16 or f16).  Tokens of q, k and v are q_stride, k_stride and
  * v_stride elements apart (multiples of 8); everything else is dense; device
  * arrays of 16-bit elements are 16-byte aligned.  lam is [lam_count] in
  * lam_dtype (dtype or SC_F32), lam_count 1 or heads; lam NULL means lam_value
  * for every head.  cu_seqlens_q / cu_seqlens_kv are HOST arrays of batch + 1
- * non-decreasing offsets starting at 0. */
+ * non-decreasing offsets starting at 0: sequences lie one behind the other
+ * without gaps, a key / value cache too. */
 typedef struct sc_diff_attention_args {
   const void *q, *k, *v, *lam;
   int64_t q_stride, k_stride, v_stride;
@@ -341,8 +342,9 @@ typedef struct sc_diff_attention_args {
 } sc_diff_attention_args;
 
 /* f32 accumulation and softmax statistics; weights and score gradients are
- * rounded to dtype for the tensor cores.  Sums have a fixed order: results
- * repeat bit for bit. */
+ * rounded to dtype for the tensor cores (in f16 scaled into its range by powers
+ * of two).  Sums have a fixed order: results repeat bit for bit.  f16 backward:
+ * rows whose log-sum-exp / scale is beyond 6.7e7 give NaN. */
 SC_API sc_status sc_diff_attention(sc_handle* h, const sc_diff_attention_args* args);
 SC_API sc_status sc_diff_attention_backward(sc_handle* h, const sc_diff_attention_args* args);
 

@@ -274,11 +274,14 @@ def sparse_diff_attention(q, k, v, lam, cu_seqlens_q, cu_seqlens_kv=None, scale=
     defaults to the former); ``scale`` (2^-20 to 2^20) defaults to ``1 / sqrt(64)``.  With
     ``causal`` query i of a sequence sees the keys ``j <= i + len_kv - len_q``
     (a single new token sees the whole cache).  Rows that see no key are zero.
-    A NaN or an infinity stays inside its sequence; there it reaches rows that
-    ``causal`` hides it from too (0 * NaN), as in any product with the weights.
-    Returns ``(total_N, H, 128)``.
+    A NaN or an infinity stays inside its sequence and makes the rows that see
+    it non-finite as softmax does; it may reach rows that ``causal`` hides it
+    from too (0 * NaN), as in any product with the weights.  Sums and softmax
+    statistics are f32; weights and score gradients are rounded to q's dtype
+    for the products.  Returns ``(total_N, H, 128)``.
 
-    Differentiable in q, k, v and lam.  ``out`` receives the result without
+    Differentiable in q, k, v and lam (f16: rows whose log-sum-exp over
+    ``scale`` is beyond 6.7e7 get NaN gradients).  ``out`` receives the result without
     autograd and may not overlap an input."""
     if q.dtype not in (torch.bfloat16, torch.float16):
         raise TypeError("sparse_diff_attention takes bf16 or f16 tensors")

@@ -4,7 +4,9 @@
 //   out[i, h] = O_1 - lam_h O_2,  O_m = softmax_j(scale Q_m[i] . K_m[j]) V[j],
 // Q_m = q[:, 2h + m], K_m = k[:, 2g + m], V = v[:, g], g = h / (heads / kv_heads).
 // Sums and softmax statistics are f32; the weights are rounded to the input
-// type for the second product.
+// type for the second product (f32 weights would halve its rate at least; the
+// output's own rounding is as large).  NaN and +inf scores, and rows whose scores
+// are all -inf, give NaN as softmax does; rows without keys are zero.
 //
 // One CTA per (tile of 128 rows, key / value head, range of keys).  A row is a
 // (token, head) pair: the heads that share a key / value head lie side by side

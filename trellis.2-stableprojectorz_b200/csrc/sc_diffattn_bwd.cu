@@ -12,8 +12,10 @@
 // keys for dK and dV) and walks tiles of the other side Y.  Both maps share dP,
 // and dV takes one product with the combined weights, so a pair of rows costs
 // 768 flops in the dQ kernel and 1024 in the other.  Accumulating dQ in the
-// dK / dV kernel instead would save the second recomputation, but needs sums
-// across CTAs whose order changes from run to run.
+// dK / dV kernel instead would save the second recomputation (1,280 in all).  It
+// was not tried: dQ would be summed across CTAs, in a fixed order only if each
+// waits for its turn at a query tile, and its products have no tensor memory left
+// there (Cfg).
 //   warp 0     TMA producer: X's Q / K pair and its dO / V once, then Y's tiles
 //              (and, for keys, the queries' statistics) into a ring
 //   warp 1     issues S_m = X_m Y_m^T and dP into tensor memory
@@ -44,8 +46,8 @@
 // times max(1, |lam|) below 2^15; in the dK / dV kernel, whose rows sum over
 // queries, dS get one for the sequence and its key / value head, and P - lam P_2
 // one that takes 1 + |lam| there.  The factors of P are added to its exponent.
-// k_da_top takes the norms' maxima.  8,192 keys, dO of 2^-14: dq off by 0.059
-// relative without, as the rounding of its result alone (0.006) with the factors.
+// k_da_top takes the norms' maxima.  8,192 keys, dO of 2^-14: dq is off by 0.067
+// relative without the factors, with them by the rounding of its result (0.0074).
 // Few CTAs: the walk is cut into ranges whose f32 sums k_da_bwd_join adds in order.
 // Every mbarrier wait is bounded (SC_ETIMEOUT).
 #include "sc_diffattn_dev.cuh"

@@ -113,7 +113,8 @@ __device__ __forceinline__ F2 neg_f2(F2 a) { return a ^ 0x8000000080000000ull; }
 
 // 1 / (1 + e^-z) of a pair, with one reciprocal for both: the special function
 // unit is what this arithmetic waits for.  e^-z is cut at 2^60, so that the
-// product of both denominators stays finite (sigmoid >= 2^-60).
+// product of both denominators stays finite: sigmoid >= 2^-60, which below
+// z = -41 puts silu(z) off by at most 2^-60 |z|.
 __device__ __forceinline__ F2 sigmoid_f2(F2 z) {
   float a, b;
   f2_split(mul_f2(z, f2(-1.4426950408889634f, -1.4426950408889634f)), a, b);
