@@ -58,7 +58,7 @@ constexpr uint32_t kColP = 128, kColO = 256;  // + 64 m, + 128 m
 constexpr float kRescale = 8.f;            // log2
 // f16 weights are written 2^7 times larger, between 2^7 and 2^15 where they are
 // largest: f16 has steps of 2^-24 at least, so unlifted it drops keys below 2^-25
-// of the row's largest weight, which 100,000 keys can make a hundredth of a row.
+// of the row's largest weight, of which 100,000 can make 0.3% of a row.
 template <typename T> constexpr float kLift = std::is_same_v<T, __half> ? 7.f : 0.f;
 
 struct DaFwd {
